@@ -51,7 +51,10 @@ enum jla_kind {              /* src/jla/ops/__init__.py:47-60 (KINDS) */
  * channel and a write gate w per value channel) is KDA with beta = 1, the values w * v and a separate read key
  * b * k: see jla_problem.k_read. */
 
-enum jla_dtype { JLA_DTYPE_BF16 = 0, JLA_DTYPE_F16 = 1, JLA_DTYPE_F32 = 2 };
+enum jla_dtype { JLA_DTYPE_BF16 = 0, JLA_DTYPE_F16 = 1, JLA_DTYPE_F32 = 2,
+                 JLA_DTYPE_E4M3 = 3 /* operands of jla_linear_fwd and jla_gated_linear_fwd only */ };
+
+enum jla_activation { JLA_ACT_NONE = 0, JLA_ACT_SILU = 1, JLA_ACT_GELU = 2 /* tanh form */, JLA_ACT_SIGMOID = 3 };
 
 enum jla_path {
   JLA_PATH_AUTO = 0,      /* f32 tensors: RECURRENT; bf16/f16: CHUNKED where it applies (KDA: K = V = 128).
@@ -262,6 +265,54 @@ int jla_gated_rmsnorm_bwd(int dtype, int64_t rows, int dim, int group, const voi
                           float eps, int sigmoid_gate, int norm_before_gate, const void* dy, void* dx, void* dz,
                           float* dweight, jla_stream_t stream);
 
+/* RMS norm of the residual stream in front of a mixer or a feed-forward block, forward and backward in one pass each:
+ *   t = x + residual (residual may be NULL), stream_out = round(t);  y = t * rsqrt(mean(t^2) + eps) * weight
+ *   out_e4m3: y is e4m3 [rows, dim] with one scale a row: scale = max |y| / 448 (1 where that is no positive normal
+ *   number), y holds value / scale
+ * x, residual, y, stream_out [rows, dim] dtype (any of the three); weight [dim] f32; scale [rows] f32; rstd [rows] f32 is
+ * written for the backward call, or NULL. 1 <= dim <= 16384.
+ * Backward: x, residual, weight as forward; dy, dstream (NULL = zero) and dx [rows, dim] dtype; dx is the gradient of x and
+ * of the residual alike; dweight [dim] f32 or NULL; scratch of jla_rms_norm_bwd_scratch_bytes() where
+ * dweight is wanted. Sums are taken in the same order every time. */
+int jla_rms_norm_fwd(int dtype, int64_t rows, int dim, const void* x, const void* residual, const float* weight, float eps,
+                     int out_e4m3, void* y, void* stream_out, float* rstd, float* scale, jla_stream_t stream);
+size_t jla_rms_norm_bwd_scratch_bytes(int64_t rows, int dim);
+int jla_rms_norm_bwd(int dtype, int64_t rows, int dim, const void* x, const void* residual, const float* rstd,
+                     const float* weight, const void* dy, const void* dstream, void* dx, float* dweight, void* scratch, size_t scratch_bytes,
+                     jla_stream_t stream);
+
+/* The projections around a mixer, with everything that follows the product in its epilogue:
+ *   z = (x W^T) * x_scale[row] * w_scale[column] + bias;  y = act(z) + residual
+ * x [rows, in] with x_stride elements between rows, w [out, in]: both BF16, both F16, or both E4M3 (then with x_scale
+ * [rows] and w_scale [out] f32, else NULL); bias [out] f32 or NULL; y and residual (or NULL) [rows, out] out_dtype (BF16 or
+ * F16; the operands' type unless they are E4M3). z [rows, out] f32 is written where it is not NULL (for the backward
+ * pass). `in` is a multiple of 8 (E4M3: of 16), `out` of 8; all pointers are 16-byte aligned, x_stride a multiple of 16
+ * bytes. Products are summed in float32.
+ * jla_gated_linear_fwd: h = act(g) * u with g = x Wg^T, u = x Wu^T (scaled alike); g and u f32, both or neither NULL.
+ * Each call is one launch. */
+int jla_linear_fwd(int dtype, int out_dtype, int64_t rows, int in, int out, const void* x, int64_t x_stride, const void* w,
+                   const float* x_scale, const float* w_scale, const float* bias, int act, const void* residual, void* y,
+                   float* z, jla_stream_t stream);
+int jla_gated_linear_fwd(int dtype, int out_dtype, int64_t rows, int in, int out, const void* x, int64_t x_stride,
+                         const void* w_gate, const void* w_up, const float* x_scale, const float* gate_scale,
+                         const float* up_scale, int act, void* h, float* g, float* u, jla_stream_t stream);
+
+/* Their backward passes (BF16 and F16), from the gradients dz [rows, out] of what the products gave:
+ *   activation:  dz = dy act'(z), dbias = sum over rows of dz (before its rounding). z NULL: dz = dy, only dbias is made (dz
+ *                may be NULL). dbias NULL: not made. scratch: jla_activation_bwd_scratch_bytes(), where dbias is wanted
+ *   gated:       dg = dh u act'(g), du = dh act(g)
+ *   input:       dx [rows, in] = dz W, or dz W + dz2 W2 (gated; w2 and dz2 NULL without)
+ *   weight:      dw [out, in] = dz^T x, and dw2 = dz2^T x in the same launch (gated; NULL without) */
+size_t jla_activation_bwd_scratch_bytes(int64_t rows, int out);
+int jla_activation_bwd(int dtype, int64_t rows, int out, int act, const float* z, const void* dy, void* dz, float* dbias,
+                       void* scratch, size_t scratch_bytes, jla_stream_t stream);
+int jla_gated_activation_bwd(int dtype, int64_t rows, int out, int act, const float* g, const float* u, const void* dh,
+                             void* dg, void* du, jla_stream_t stream);
+int jla_linear_bwd_input(int dtype, int64_t rows, int in, int out, const void* dz, const void* w, const void* dz2,
+                         const void* w2, void* dx, jla_stream_t stream);
+int jla_linear_bwd_weight(int dtype, int64_t rows, int in, int out, const void* dz, const void* dz2, const void* x,
+                          int64_t x_stride, void* dw, void* dw2, jla_stream_t stream);
+
 /* Diagnostics: where the chunked path keeps its intermediates, so that tests can compare them stage by stage
  * with the CPU model (the reference checks its kernels per stage too:
  * tests/test_mosaic_gpu_gated_delta_rule.py:104-146). Byte offsets into the residual buffer written by a forward
@@ -316,7 +367,8 @@ int jla_piece_scan(int backward, int P, int H, int K, int V, const float* maps, 
  * word that lives on the GPU (one word per GPU that loads the library), and the results of that launch are
  * undefined. jla_device_status() waits for `stream`, copies the word of the CURRENT device to *out and clears it:
  * 0 = every launch since the last query completed its waits; 1 = a chunk-gradient kernel, 2 = a forward state
- * pass, 3 = a reverse state pass gave up; 9 = jla_selftest_bounded_wait. It blocks the host (diagnostic call; the
+ * pass, 3 = a reverse state pass, 4 = a matrix product, 5 = a product of few tokens gave up; 9 =
+ * jla_selftest_bounded_wait. It blocks the host (diagnostic call; the
  * compute entry points never do). No counterpart in the reference, whose Pallas kernels wait without a bound. */
 int jla_device_status(int* out, jla_stream_t stream);
 

@@ -98,9 +98,20 @@ def load() -> C.CDLL:
         "jla_ssd_output_fwd": [int_, i64, int_, int_] + [ptr] * 5, "jla_ssd_output_bwd": [int_, i64, int_, int_] + [ptr] * 6,
         "jla_ssd_layer_bwd": [int_, i64, int_, int_] + [ptr] * 12,
         "jla_ssd_step": [C.POINTER(Problem)] + [ptr] * 6,
+        "jla_rms_norm_fwd": [int_, i64, int_] + [ptr] * 3 + [f32, int_] + [ptr] * 5,
+        "jla_rms_norm_bwd": [int_, i64, int_] + [ptr] * 9 + [C.c_size_t, ptr],
+        "jla_linear_fwd": [int_, int_, i64, int_, int_, ptr, i64] + [ptr] * 4 + [int_] + [ptr] * 4,
+        "jla_gated_linear_fwd": [int_, int_, i64, int_, int_, ptr, i64] + [ptr] * 5 + [int_] + [ptr] * 4,
+        "jla_activation_bwd": [int_, i64, int_, int_] + [ptr] * 5 + [C.c_size_t, ptr],
+        "jla_gated_activation_bwd": [int_, i64, int_, int_] + [ptr] * 6,
+        "jla_linear_bwd_input": [int_, i64, int_, int_] + [ptr] * 6,
+        "jla_linear_bwd_weight": [int_, i64, int_, int_] + [ptr] * 3 + [i64] + [ptr] * 3,
     }.items():
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = C.c_int, types
+    for name in ("jla_rms_norm_bwd_scratch_bytes", "jla_activation_bwd_scratch_bytes"):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = C.c_size_t, [i64, int_]
     lib.jla_device_status.restype = C.c_int
     lib.jla_device_status.argtypes = [C.POINTER(C.c_int), C.c_void_p]
     lib.jla_selftest_bounded_wait.restype = C.c_int

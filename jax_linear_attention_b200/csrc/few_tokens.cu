@@ -1,0 +1,311 @@
+// Matrix products of few tokens (a decoding step, a short prompt) with the epilogue fused: the same results as
+// product_tc.cu, for calls whose time is that of reading the weights.
+//
+// Bound by HBM, so the weights have to stream through as many SMs as there are. The roles of the operands are swapped: 128
+// features (rows of W) fill the 128 TMEM lanes, BN tokens are the accumulator's columns, so that few tokens waste
+// neither tensor-core rows nor shared memory. The contraction is cut into up to eight parts, one for each CTA of a
+// cluster; each CTA leaves its partial sums in shared memory, and the cluster's CTAs share out the tokens among
+// themselves and add the parts up over distributed shared memory, in the order of the parts, every time the same.
+//
+// A thread of the epilogue holds one feature, so a warp's stores of one token are 32 neighbouring elements.
+//
+// Every wait is bounded, as in product_tc.cu (kStatusFewTokens).
+#include "product.cuh"
+#include "profile.cuh"
+#include "umma_pair.cuh"
+
+namespace jla {
+namespace {
+
+using umma::smem_addr;
+
+constexpr int kThreads = 192;  // warps 0 .. 3 epilogue, 4 loads, 5 products
+constexpr int kMaxSplit = 8;
+
+struct Maps {
+  CUtensorMap x[2], w[2];
+};
+
+struct Params {
+  int rows, features;
+  int kt0, kt;
+  uint32_t idesc;
+  int act, half;
+  const float *x_scale, *w_scale[2], *bias;
+  const void* residual;
+  void* y;
+  float* save[2];
+  int* status;
+};
+
+template <int BN, bool GATED> struct Shape {
+  static constexpr int kWeightBytes = 128 * 128;
+  static constexpr int kStageBytes = (GATED ? 2 : 1) * kWeightBytes + BN * 128;
+  // up to 12 stages, 200 KB at most; the partial sums lie in the same memory afterwards
+  static constexpr int kFit = 200 * 1024 / kStageBytes;
+  static constexpr int kStages = kFit < 12 ? kFit : 12;
+  static constexpr int kPartBytes = (GATED ? 2 : 1) * BN * 128 * 4;
+  static constexpr int kRing = kStages * kStageBytes;
+  static constexpr int kSmem = (kRing > kPartBytes ? kRing : kPartBytes) + 1024;
+  // TMEM columns: a load takes 32 from the start of an accumulator, also where the accumulator has 16
+  static constexpr int kNeed = (GATED ? BN : 0) + (BN < 32 ? 32 : BN);
+  static constexpr int kCols = kNeed <= 32 ? 32 : kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : 256;
+};
+
+// What is left of a feature's value at one token after the products: scales, bias, activation, residual, store.
+template <bool FP8, bool GATED>
+__device__ __forceinline__ void finish(const Params& p, int token, int f, float v, float u, float ws0, float ws1, float bias) {
+  const size_t at = (size_t)token * p.features + f;
+  if constexpr (FP8) {
+    const float xs = __ldg(p.x_scale + token);
+    v *= xs * ws0;
+    if constexpr (GATED) u *= xs * ws1;
+  }
+  if constexpr (GATED) {
+    if (p.save[0]) p.save[0][at] = v, p.save[1][at] = u;
+    v = activate(p.act, v) * u;
+  } else {
+    v += bias;
+    if (p.save[0]) p.save[0][at] = v;
+    v = activate(p.act, v);
+    if (p.residual) {
+      v += p.half ? __half2float(__ldg(static_cast<const __half*>(p.residual) + at))
+                  : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.residual) + at));
+    }
+  }
+  if (p.half) static_cast<__half*>(p.y)[at] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
+}
+
+template <int BN, bool W_MN, bool FP8, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1) few_tokens_kernel(const __grid_constant__ Maps maps,
+                                                                 const __grid_constant__ Params p, int split) {
+  using S = Shape<BN, GATED>;
+  constexpr int ST = S::kStages, NW = GATED ? 2 : 1;
+  extern __shared__ unsigned char smem_dyn[];
+  __shared__ __align__(8) uint64_t full[ST], empty[ST], done, drain;
+  __shared__ uint32_t tmem_slot;
+  const uint32_t base = (smem_addr(smem_dyn) + 1023) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = split > 1 ? (int)umma::cluster_rank() : 0;
+  const int f0 = (int)(blockIdx.x / split) * 128, m0 = (int)blockIdx.y * BN;
+  const int k_lo = (int)((long)p.kt * part / split), k_hi = (int)((long)p.kt * (part + 1) / split);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      umma::mbar_init(full + i, 1);
+      umma::mbar_init(empty + i, 1);
+    }
+    umma::mbar_init(&done, 1);
+    umma::mbar_init(&drain, 1);
+    umma::mbar_init_fence();
+  }
+  if (warp == 5) umma::tmem_alloc(&tmem_slot, S::kCols);
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  bool ok = true;
+
+  if (warp == 4 && lane == 0) {
+    int it = 0;
+    for (int kt = k_lo; kt < k_hi; ++kt, ++it) {
+      const int s = it % ST;
+      if (it >= ST) ok = umma::mbar_wait(empty + s, ((it / ST) - 1) & 1);
+      if (!ok) break;
+      tma::expect_tx(full + s, S::kStageBytes);
+      const uint32_t bar = smem_addr(full + s);
+      const bool second = kt >= p.kt0;
+      const int k0 = (second ? kt - p.kt0 : kt) * (FP8 ? 128 : 64);
+      const uint32_t ws = base + s * S::kStageBytes, xs = ws + NW * S::kWeightBytes;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        const CUtensorMap* mw = &maps.w[GATED ? i : (second ? 1 : 0)];
+        if constexpr (W_MN) {
+          tma::load_2d(ws + i * S::kWeightBytes, mw, f0, k0, bar);
+          tma::load_2d(ws + i * S::kWeightBytes + 8192, mw, f0 + 64, k0, bar);
+        } else {
+          tma::load_2d(ws + i * S::kWeightBytes, mw, k0, f0, bar);
+        }
+      }
+      tma::load_2d(xs, &maps.x[second ? 1 : 0], k0, m0, bar);
+    }
+    if (!ok) {
+      for (int j = it > ST ? it - ST : 0; j < it; ++j) umma::mbar_wait(full + j % ST, (j / ST) & 1);
+    }
+  } else if (warp == 5 && lane == 0) {
+    const uint64_t w0 = umma::smem_desc(base, W_MN ? 8192 : 16, 1024);
+    const uint64_t x0 = umma::smem_desc(base + NW * S::kWeightBytes, 16, 1024);
+    int it = 0;
+    for (int kt = k_lo; kt < k_hi; ++kt, ++it) {
+      const int s = it % ST;
+      ok = umma::mbar_wait(full + s, (it / ST) & 1);
+      if (!ok) break;
+      umma::fence_after_sync();
+      const uint32_t off = (uint32_t)(s * S::kStageBytes) >> 4;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          umma::mma_any<FP8>(tmem + i * BN, w0 + off + i * (S::kWeightBytes >> 4) + (W_MN ? ks * 128 : ks * 2),
+                             x0 + off + ks * 2, p.idesc, it > 0 || ks > 0);
+        }
+      }
+      umma::commit(empty + s);
+    }
+    if (ok) {
+      umma::commit(&done);
+    } else {
+      umma::commit(&drain);
+      umma::mbar_wait(&drain, 0);
+    }
+  }
+  if (warp < 4) {
+    ok = umma::mbar_wait(&done, 0);
+    umma::fence_after_sync();
+  }
+  const int f = f0 + warp * 32 + lane;  // (warps 0 .. 3)
+  const uint32_t acc = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+  const int tokens = p.rows - m0 < BN ? p.rows - m0 : BN;
+  float ws0 = 0.f, ws1 = 0.f, bias = 0.f;
+  if (warp < 4 && f < p.features) {
+    if constexpr (FP8) {
+      ws0 = __ldg(p.w_scale[0] + f);
+      if constexpr (GATED) ws1 = __ldg(p.w_scale[1] + f);
+    }
+    if (p.bias) bias = __ldg(p.bias + f);
+  }
+  constexpr int CH = BN < 32 ? BN : 32;  // columns a step (16: the last 16 of a load are not looked at)
+  if (split == 1) {
+    if (warp < 4 && __all_sync(0xffffffffu, ok)) {
+#pragma unroll 1
+      for (int c = 0; c < tokens; c += CH) {
+        float v[32], u[32];
+        umma::ld_32x32b_x32(v, acc + c);
+        if constexpr (GATED) umma::ld_32x32b_x32(u, acc + BN + c);
+        umma::wait_ld();
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          if (c + i < tokens && f < p.features) finish<FP8, GATED>(p, m0 + c + i, f, v[i], GATED ? u[i] : 0.f, ws0, ws1, bias);
+        }
+      }
+    }
+  } else {
+    // partial sums [weight][token][128 features] over the ring, which is idle now
+    if (warp < 4 && __all_sync(0xffffffffu, ok)) {
+#pragma unroll 1
+      for (int c = 0; c < tokens; c += CH) {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+          float v[32];
+          umma::ld_32x32b_x32(v, acc + i * BN + c);
+          umma::wait_ld();
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            if (c + j < tokens) {
+              asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(base + ((i * BN + c + j) * 128 + warp * 32 + lane) * 4), "f"(v[j])
+                           : "memory");
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    umma::cluster_sync();
+    if (warp < 4 && f < p.features) {
+      for (int c = part; c < tokens; c += split) {
+        float sum[NW];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+          const uint32_t at = base + ((i * BN + c) * 128 + warp * 32 + lane) * 4;
+          float v[kMaxSplit];
+#pragma unroll
+          for (int r = 0; r < kMaxSplit; ++r) v[r] = r < split ? umma::ld_cluster(umma::map_rank(at, r)) : 0.f;
+          sum[i] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        }
+        finish<FP8, GATED>(p, m0 + c, f, sum[0], GATED ? sum[NW - 1] : 0.f, ws0, ws1, bias);
+      }
+    }
+    __syncwarp();
+    umma::cluster_sync();  // the others read this CTA's part until here
+  }
+  if (!ok) atomicExch(p.status, kStatusFewTokens);
+  umma::fence_before_sync();
+  __syncthreads();
+  if (warp == 5) umma::tmem_dealloc(tmem, S::kCols);
+}
+
+// Parts of the contraction: as many as keep every SM at work, each of at least two steps.
+int parts(int tiles, int kt, int sms) {
+  int s = sms / tiles;
+  if (s > kt / 2) s = kt / 2;
+  return s < 1 ? 1 : (s > kMaxSplit ? kMaxSplit : s);
+}
+
+template <int BN, bool W_MN, bool FP8, bool GATED>
+int launch(const Product& p, int sms, cudaStream_t s) {
+  using S = Shape<BN, GATED>;
+  Maps maps;
+  Params q{};
+  const int esz = FP8 ? 1 : 2, kb = FP8 ? 128 : 64;
+  bool ok = true;
+  for (int i = 0; i < 2 && ok; ++i) {
+    const void *x = p.x[i] ? p.x[i] : p.x[0], *w = p.w[i] ? p.w[i] : p.w[0];
+    ok = tma::encode_2d(&maps.x[i], x, esz, p.depth, p.rows, p.x_stride, BN) &&
+         (W_MN ? tma::encode_2d(&maps.w[i], w, esz, p.features, p.depth, p.w_stride, 64)
+               : tma::encode_2d(&maps.w[i], w, esz, p.depth, p.features, p.w_stride, 128));
+  }
+  if (!ok) return JLA_ERR_CUDA;
+  q.rows = (int)p.rows, q.features = p.features;
+  q.kt0 = (p.depth + kb - 1) / kb;
+  q.kt = q.kt0 * (p.pair ? 2 : 1);
+  q.idesc = FP8 ? umma::instr_desc_e4m3(128, BN) : umma::instr_desc(128, BN, p.dtype == JLA_DTYPE_BF16, W_MN, 0);
+  q.act = p.act, q.half = p.out_dtype == JLA_DTYPE_F16;
+  q.x_scale = p.x_scale, q.w_scale[0] = p.w_scale[0], q.w_scale[1] = p.w_scale[1], q.bias = p.bias, q.residual = p.residual;
+  q.y = p.y[0], q.save[0] = p.save[0], q.save[1] = p.save[1];
+  q.status = tc_status_ptr();
+  if (!q.status) {
+    set_error("the status word of the current device could not be located");
+    return JLA_ERR_CUDA;
+  }
+  const int tiles_f = (p.features + 127) / 128, tiles_m = (int)((p.rows + BN - 1) / BN);
+  int split = parts(tiles_f * tiles_m, q.kt, sms);
+  auto* kern = few_tokens_kernel<BN, W_MN, FP8, GATED>;
+  JLA_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(tiles_f * split, tiles_m), cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem, cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = split, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  {
+    ProfScope scope(kProfFewTokens, s);
+    JLA_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, maps, q, split));
+  }
+  JLA_LAUNCH_OK();
+  return JLA_OK;
+}
+
+template <bool W_MN, bool FP8, bool GATED>
+int pick(const Product& p, cudaStream_t s) {
+  int dev = 0, sms = 0;
+  JLA_CUDA_OK(cudaGetDevice(&dev));
+  JLA_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  if (p.rows <= 16) return launch<16, W_MN, FP8, GATED>(p, sms, s);
+  if (p.rows <= 32) return launch<32, W_MN, FP8, GATED>(p, sms, s);
+  if (p.rows <= 64) return launch<64, W_MN, FP8, GATED>(p, sms, s);
+  return launch<128, W_MN, FP8, GATED>(p, sms, s);
+}
+
+}  // namespace
+
+bool few_tokens_applies(const Product& p) { return !p.x_mn && !p.group && p.rows <= 256; }
+
+int product_few_tokens(const Product& p, cudaStream_t s) {
+  if (p.dtype == JLA_DTYPE_E4M3) return p.gated ? pick<false, true, true>(p, s) : pick<false, true, false>(p, s);
+  if (p.w_mn) return pick<true, false, false>(p, s);
+  return p.gated ? pick<false, false, true>(p, s) : pick<false, false, false>(p, s);
+}
+
+}  // namespace jla

@@ -1,0 +1,80 @@
+// What the matrix-product kernels share: the activations of their epilogues, their parameters, and their launchers.
+//
+//   linear:  z = (x W^T) xs ws + bias,  y = act(z) + residual          gated:  h = act(x Wg^T xs gs) * (x Wu^T xs us)
+#pragma once
+
+#include "common.cuh"
+#include "tma.cuh"
+
+namespace jla {
+
+enum { kActNone = JLA_ACT_NONE, kActSilu = JLA_ACT_SILU, kActGelu = JLA_ACT_GELU, kActSigmoid = JLA_ACT_SIGMOID };
+
+constexpr int kStatusProduct = 4, kStatusFewTokens = 5;  // codes of the device status word
+
+__device__ __forceinline__ float sigmoid_f32(float z) { return fast_rcp(1.f + fast_exp(-z)); }
+
+// gelu in its tanh form: 0.5 z (1 + tanh(t)) = z sigmoid(2 t), t = sqrt(2 / pi) (z + 0.044715 z^3)
+constexpr float kGelu2C = 1.5957691216057308f, kGeluA = 0.044715f;
+
+__device__ __forceinline__ float activate(int act, float z) {
+  if (act == kActNone) return z;
+  const float s = sigmoid_f32(act == kActGelu ? kGelu2C * (z + kGeluA * z * z * z) : z);
+  return act == kActSigmoid ? s : z * s;
+}
+// act'(z)
+__device__ __forceinline__ float activation_slope(int act, float z) {
+  if (act == kActNone) return 1.f;
+  if (act == kActGelu) {
+    const float s = sigmoid_f32(kGelu2C * (z + kGeluA * z * z * z));
+    return s + z * s * (1.f - s) * kGelu2C * (1.f + 3.f * kGeluA * z * z);
+  }
+  const float s = sigmoid_f32(z);
+  return act == kActSigmoid ? s * (1.f - s) : s * (1.f + z * (1.f - s));
+}
+
+// Two float32 values rounded to bf16 or f16 (`half`) in one register.
+__device__ __forceinline__ uint32_t pack_out(bool half, float lo, float hi) {
+  if (half) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 unpack_out(bool half, uint32_t x) {
+  return half ? __half22float2(*reinterpret_cast<const __half2*>(&x))
+              : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+}
+
+// One product (host view). "tokens" are the rows of y, "features" its columns; the contraction runs over `depth`, and over
+// the second pair of operands after the first where there is one (dx = dg Wg + du Wu).
+struct Product {
+  int dtype = 0;      // of the operands: JLA_DTYPE_BF16, _F16 or _E4M3
+  int out_dtype = 0;  // of y and the residual: JLA_DTYPE_BF16 or _F16
+  int64_t rows = 0;
+  int features = 0, depth = 0;
+  bool gated = false;    // two weights, two accumulators a column
+  bool pair = false;     // a second pair of operands in the contraction
+  bool group = false;    // a second product with operands x[1] and w[0], written to y[1]
+  bool x_mn = false, w_mn = false;  // operand stored with the contraction along its rows ([depth][tokens], [depth][features])
+  const void* x[2] = {};
+  int64_t x_stride = 0;  // elements between the rows of x in memory
+  const void* w[2] = {};
+  int64_t w_stride = 0;
+  const float* x_scale = nullptr;
+  const float* w_scale[2] = {};
+  const float* bias = nullptr;
+  int act = 0;
+  const void* residual = nullptr;
+  void* y[2] = {};
+  float* save[2] = {};   // z, or g and u, in float32 for a later backward pass
+};
+
+int product_pairs(const Product& p, cudaStream_t stream);       // product_tc.cu: any number of tokens
+int product_few_tokens(const Product& p, cudaStream_t stream);  // few_tokens.cu: at most kFewTokens
+bool few_tokens_applies(const Product& p);
+
+int* tc_status_ptr();  // status.cu
+
+}  // namespace jla

@@ -1,0 +1,390 @@
+// Matrix products of any number of tokens on pairs of CTAs (tcgen05.mma.cta_group::2), with the epilogue fused:
+//
+//   linear   y = act((x W^T) xs ws + bias) + residual      (z before the activation in float32 for a backward pass)
+//   gated    h = act(g) u,  g = x Wg^T,  u = x Wu^T          (g and u in float32 for a backward pass)
+//   dx       = dz W, or dg Wg + du Wu                        (W read with the contraction along its rows)
+//   dW       = dz^T x, or two of them in one launch          (both operands with the contraction along their rows)
+//
+// Bound by the tensor cores. A persistent pair of CTAs takes tiles of 256 rows and BN columns (BN / 2 columns of each
+// weight where gated): a warp fetches operand tiles of 128 bytes of contraction by TMA into a ring of 6 or 8 stages, one
+// thread of the leading CTA issues the products, four warps of each CTA take finished accumulators out of TMEM (32 rows a
+// warp, a row a thread) through shared memory and TMA stores. Two sets of accumulators: the epilogue of one tile
+// runs under the products of the next. A pair reads an operand byte from L2 half as often as two CTAs of 128 x BN would.
+//
+// Where the operands end inside a tile TMA reads zeros and its stores leave out what lies beyond. No load is multicast.
+// Every wait is bounded: one that runs out records kStatusProduct, and the kernel lets its copies and products in flight
+// finish, frees its TMEM and returns.
+#include "product.cuh"
+#include "profile.cuh"
+#include "umma_pair.cuh"
+
+namespace jla {
+namespace {
+
+using umma::smem_addr;
+
+constexpr int kThreads = 256;  // warps: 0 loads, 1 products, 2 TMEM, 3 none, 4 .. 7 epilogue
+constexpr int kStagingWarp = 2 * 4096;  // two boxes of 32 rows x 128 bytes for each epilogue warp
+
+struct Maps {
+  CUtensorMap x[2], w[2], y[2], save[2];
+};
+
+struct Params {
+  int rows, features;           // of y
+  int tiles_n, tiles_mn, tiles; // tiles in a row of tiles, in one product, in all
+  int kt0, kt;                  // steps of the contraction with the first pair of operands, and in all
+  uint32_t idesc;
+  int act, half, saves;
+  const float *x_scale, *w_scale[2], *bias;
+  const void* residual;
+  int* status;
+};
+
+template <int BN> struct Shape {
+  static constexpr int kStageBytes = 128 * 128 + BN / 2 * 128;  // a CTA's part of both operands
+  static constexpr int kStages = BN == 256 ? 6 : 8;
+  static constexpr int kSmem = kStages * kStageBytes + 4 * kStagingWarp + 1024;
+};
+
+// Tile `t` of one product: bands of 8 columns of tiles, row after row inside a band, so that the tiles in work at one time
+// form a block whose operands stay in L2.
+__device__ __forceinline__ void locate(const Params& p, int t, int& tm, int& tn) {
+  constexpr int kBand = 8;
+  const int tiles_m = p.tiles_mn / p.tiles_n;
+  const int band = t / (kBand * tiles_m);
+  const int left = p.tiles_n - band * kBand, width = left < kBand ? left : kBand;
+  const int in = t - band * kBand * tiles_m;
+  tm = in / width;
+  tn = band * kBand + in % width;
+}
+
+// A warp's two staging boxes: 32 rows of 128 bytes, 128-byte swizzle (16-byte chunk j of row r lies at chunk j ^ (r % 8)).
+struct Staging {
+  uint32_t base;
+  int next;
+  __device__ __forceinline__ uint32_t acquire(int lane) {
+    if (lane == 0) tma::store_wait_read<1>();
+    __syncwarp();
+    const uint32_t at = base + next * 4096;
+    next ^= 1;
+    return at;
+  }
+  static __device__ __forceinline__ void put(uint32_t box, int lane, int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(box + lane * 128 + ((chunk ^ (lane & 7)) << 4)), "r"(a),
+                 "r"(b), "r"(c), "r"(d)
+                 : "memory");
+  }
+  static __device__ __forceinline__ void release(uint32_t box, int lane, const CUtensorMap* map, int col, int row, int cols,
+                                                 int rows) {
+    umma::fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (col < cols && row < rows) tma::store_2d(map, box, col, row);
+      tma::store_commit();
+    }
+  }
+  __device__ __forceinline__ void save32(const float (&v)[32], int lane, const CUtensorMap* map, int col, int row, int cols,
+                                         int rows) {
+    const uint32_t box = acquire(lane);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      put(box, lane, j, __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+          __float_as_uint(v[4 * j + 3]));
+    }
+    release(box, lane, map, col, row, cols, rows);
+  }
+  __device__ __forceinline__ void store64(const uint32_t (&v)[32], int lane, const CUtensorMap* map, int col, int row,
+                                          int cols, int rows) {
+    const uint32_t box = acquire(lane);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) put(box, lane, j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    release(box, lane, map, col, row, cols, rows);
+  }
+};
+
+// v[i] = v[i] * s * scale[col + i], for the columns inside the matrix (a multiple of 8: whole float4s)
+__device__ __forceinline__ void scale_columns(float (&v)[32], float s, const float* scale, int col, int cols) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    if (col + i < cols) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(scale + col + i));
+      v[i] *= s * f.x, v[i + 1] *= s * f.y, v[i + 2] *= s * f.z, v[i + 3] *= s * f.w;
+    }
+  }
+}
+
+template <int BN, bool X_MN, bool W_MN, bool FP8, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  using S = Shape<BN>;
+  constexpr int ST = S::kStages;
+  extern __shared__ unsigned char smem_dyn[];
+  __shared__ __align__(8) uint64_t full[ST], empty[ST], acc_full[2], acc_empty[2], drain;
+  __shared__ uint32_t tmem_slot;
+  const uint32_t base = (smem_addr(smem_dyn) + 1023) & ~1023u;
+  const uint32_t staging = base + ST * S::kStageBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = umma::cluster_rank();
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      umma::mbar_init(full + i, 1);
+      umma::mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      umma::mbar_init(acc_full + i, 1);
+      umma::mbar_init(acc_empty + i, 8);  // the epilogue warps of both CTAs
+    }
+    umma::mbar_init(&drain, 1);
+    umma::mbar_init_fence();
+  }
+  if (warp == 2) umma::tmem_alloc_pair(&tmem_slot, 2 * BN);
+  umma::fence_before_sync();
+  umma::cluster_sync();
+  umma::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  bool ok = true;
+
+  if (warp == 0 && lane == 0) {
+    // ---- loads: this CTA's 128 rows of x and its half of the weight's; the bytes count on the leader's barrier
+    tma::prefetch_map(&maps.x[0]);
+    tma::prefetch_map(&maps.w[0]);
+    int it = 0;
+    for (int t = first; t < p.tiles && ok; t += step) {
+      const int g = t / p.tiles_mn;
+      int tm, tn;
+      locate(p, t - g * p.tiles_mn, tm, tn);
+      const int m0 = tm * 256 + (int)rank * 128;
+      const int n0 = GATED ? tn * (BN / 2) : tn * BN + (int)rank * (BN / 2);
+      for (int kt = 0; kt < p.kt && ok; ++kt, ++it) {
+        const int s = it % ST;
+        if (it >= ST) ok = umma::mbar_wait(empty + s, ((it / ST) - 1) & 1);
+        if (!ok) break;
+        if (rank == 0) tma::expect_tx(full + s, 2 * S::kStageBytes);
+        const uint32_t bar = umma::map_rank(smem_addr(full + s), 0);
+        const bool second = kt >= p.kt0;
+        const CUtensorMap* mx = &maps.x[second ? 1 : g];
+        const CUtensorMap* mw = &maps.w[GATED ? rank : (second ? 1 : 0)];
+        const int k0 = (second ? kt - p.kt0 : kt) * (FP8 ? 128 : 64);
+        const uint32_t xs = base + s * S::kStageBytes, ws = xs + 128 * 128;
+        if constexpr (X_MN) {
+          tma::load_2d_pair(xs, mx, m0, k0, bar);
+          tma::load_2d_pair(xs + 8192, mx, m0 + 64, k0, bar);
+        } else {
+          tma::load_2d_pair(xs, mx, k0, m0, bar);
+        }
+        if constexpr (W_MN) {
+#pragma unroll
+          for (int b = 0; b < BN / 128; ++b) tma::load_2d_pair(ws + b * 8192, mw, n0 + b * 64, k0, bar);
+        } else {
+          tma::load_2d_pair(ws, mw, k0, n0, bar);
+        }
+      }
+    }
+    if (!ok && rank == 0) {  // let what was asked for land before the block's memory is given up
+      for (int j = it > ST ? it - ST : 0; j < it; ++j) umma::mbar_wait(full + j % ST, (j / ST) & 1);
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---- products
+    const uint64_t x0 = umma::smem_desc(base, X_MN ? 8192 : 16, 1024);
+    const uint64_t w0 = umma::smem_desc(base + 128 * 128, W_MN ? 8192 : 16, 1024);
+    int it = 0, n = 0;
+    for (int t = first; t < p.tiles && ok; t += step, ++n) {
+      const int a = n & 1;
+      if (n >= 2) ok = umma::mbar_wait(acc_empty + a, ((n >> 1) - 1) & 1);
+      umma::fence_after_sync();
+      for (int kt = 0; kt < p.kt && ok; ++kt, ++it) {
+        const int s = it % ST;
+        ok = umma::mbar_wait(full + s, (it / ST) & 1);
+        if (!ok) break;
+        umma::fence_after_sync();
+        const uint32_t off = (uint32_t)(s * S::kStageBytes) >> 4;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          umma::mma_pair<FP8>(tmem + a * BN, x0 + off + (X_MN ? ks * 128 : ks * 2), w0 + off + (W_MN ? ks * 128 : ks * 2),
+                              p.idesc, kt > 0 || ks > 0);
+        }
+        umma::commit_pair(empty + s);
+      }
+      if (ok) umma::commit_pair(acc_full + a);
+    }
+    if (!ok) {  // products in flight read both CTAs' shared memory: wait for them
+      umma::commit_pair(&drain);
+      umma::mbar_wait(&drain, 0);
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue: warp w owns the TMEM lanes (rows) 32 w .. 32 w + 31 of its CTA
+    const int w = warp & 3;
+    Staging stage{staging + (uint32_t)w * kStagingWarp, 0};
+    const bool half = p.half;
+    int n = 0;
+    for (int t = first; t < p.tiles; t += step, ++n) {
+      const int a = n & 1;
+      ok = umma::mbar_wait(acc_full + a, (n >> 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      umma::fence_after_sync();
+      const int g = t / p.tiles_mn;
+      int tm, tn;
+      locate(p, t - g * p.tiles_mn, tm, tn);
+      const int row0 = tm * 256 + (int)rank * 128 + w * 32, row = row0 + lane;
+      const bool live = row < p.rows;
+      const uint32_t acc = tmem + a * BN + ((uint32_t)(32 * w) << 16);
+      float xs = 1.f;
+      if constexpr (FP8) xs = live ? __ldg(p.x_scale + row) : 0.f;
+      constexpr int COLS = GATED ? BN / 2 : BN;
+#pragma unroll 1
+      for (int c = 0; c < COLS; c += 64) {
+        const int col = tn * COLS + c;
+        if (col >= p.features || row0 >= p.rows) break;
+        uint32_t out[32];
+        uint4 res[8];
+        if (!GATED && p.residual) {
+          const uint4* r = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + (size_t)row * p.features + col);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) res[j] = live && col + 8 * j < p.features ? __ldg(r + j) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int hc = col + 32 * h;
+          float v[32];
+          umma::ld_32x32b_x32(v, acc + c + 32 * h);
+          if constexpr (GATED) {
+            float u[32];
+            umma::ld_32x32b_x32(u, acc + BN / 2 + c + 32 * h);
+            umma::wait_ld();
+            if constexpr (FP8) {
+              scale_columns(v, xs, p.w_scale[0], hc, p.features);
+              scale_columns(u, xs, p.w_scale[1], hc, p.features);
+            }
+            if (p.saves) {
+              stage.save32(v, lane, &maps.save[0], hc, row0, p.features, p.rows);
+              stage.save32(u, lane, &maps.save[1], hc, row0, p.features, p.rows);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = activate(p.act, v[i]) * u[i];
+          } else {
+            umma::wait_ld();
+            if constexpr (FP8) scale_columns(v, xs, p.w_scale[0], hc, p.features);
+            if (p.bias) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                if (hc + i < p.features) {
+                  const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + hc + i));
+                  v[i] += b.x, v[i + 1] += b.y, v[i + 2] += b.z, v[i + 3] += b.w;
+                }
+              }
+            }
+            if (p.saves) stage.save32(v, lane, &maps.save[0], hc, row0, p.features, p.rows);
+            if (p.act != kActNone) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = activate(p.act, v[i]);
+            }
+            if (p.residual) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint4 q = res[4 * h + j];
+                const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float2 f = unpack_out(half, e[i]);
+                  v[8 * j + 2 * i] += f.x, v[8 * j + 2 * i + 1] += f.y;
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) out[16 * h + i] = pack_out(half, v[2 * i], v[2 * i + 1]);
+        }
+        stage.store64(out, lane, &maps.y[g], col, row0, p.features, p.rows);
+      }
+      umma::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) umma::arrive_cluster(umma::map_rank(smem_addr(acc_empty + a), 0));
+    }
+    if (lane == 0) tma::store_wait<0>();
+  }
+  if (!ok) atomicExch(p.status, kStatusProduct);
+  __syncthreads();
+  umma::fence_before_sync();
+  umma::cluster_sync();  // no product or arrival of the other CTA may still be on its way here
+  umma::fence_after_sync();
+  if (warp == 2) umma::tmem_dealloc_pair(tmem, 2 * BN);
+}
+
+template <int BN, bool X_MN, bool W_MN, bool FP8, bool GATED>
+int launch(const Product& p, int sms, cudaStream_t s) {
+  using S = Shape<BN>;
+  Maps maps;
+  Params q{};
+  const int esz = FP8 ? 1 : 2, kb = FP8 ? 128 : 64;
+  const int xr = X_MN ? 64 : 128, wr = W_MN ? 64 : BN / 2;
+  bool ok = true;
+  for (int i = 0; i < 2 && ok; ++i) {
+    const void *x = p.x[i] ? p.x[i] : p.x[0], *w = p.w[i] ? p.w[i] : p.w[0];
+    void *y = p.y[i] ? p.y[i] : p.y[0];
+    ok = (X_MN ? tma::encode_2d(&maps.x[i], x, esz, p.rows, p.depth, p.x_stride, xr)
+               : tma::encode_2d(&maps.x[i], x, esz, p.depth, p.rows, p.x_stride, xr)) &&
+         (W_MN ? tma::encode_2d(&maps.w[i], w, esz, p.features, p.depth, p.w_stride, wr)
+               : tma::encode_2d(&maps.w[i], w, esz, p.depth, p.features, p.w_stride, wr)) &&
+         tma::encode_2d(&maps.y[i], y, 2, p.features, p.rows, p.features, 32) &&
+         (!p.save[i] || tma::encode_2d(&maps.save[i], p.save[i], 4, p.features, p.rows, p.features, 32));
+  }
+  if (!ok) return JLA_ERR_CUDA;
+  constexpr int COLS = GATED ? BN / 2 : BN;
+  q.rows = (int)p.rows, q.features = p.features;
+  q.tiles_n = (p.features + COLS - 1) / COLS;
+  q.tiles_mn = (int)((p.rows + 255) / 256) * q.tiles_n;
+  q.tiles = q.tiles_mn * (p.group ? 2 : 1);
+  q.kt0 = (p.depth + kb - 1) / kb;
+  q.kt = q.kt0 * (p.pair ? 2 : 1);
+  q.idesc = FP8 ? umma::instr_desc_e4m3(256, BN) : umma::instr_desc(256, BN, p.dtype == JLA_DTYPE_BF16, X_MN, W_MN);
+  q.act = p.act, q.half = p.out_dtype == JLA_DTYPE_F16, q.saves = p.save[0] != nullptr;
+  q.x_scale = p.x_scale, q.w_scale[0] = p.w_scale[0], q.w_scale[1] = p.w_scale[1], q.bias = p.bias, q.residual = p.residual;
+  q.status = tc_status_ptr();
+  if (!q.status) {
+    set_error("the status word of the current device could not be located");
+    return JLA_ERR_CUDA;
+  }
+  auto* kern = product_kernel<BN, X_MN, W_MN, FP8, GATED>;
+  JLA_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  const int pairs = sms / 2 < q.tiles ? sms / 2 : q.tiles;
+  {
+    ProfScope scope(kProfProduct, s);
+    kern<<<2 * pairs, kThreads, S::kSmem, s>>>(maps, q);
+  }
+  JLA_LAUNCH_OK();
+  return JLA_OK;
+}
+
+// 256 columns a tile keep the tensor cores busier per operand byte; 128 columns waste less where the last round of tiles is
+// short. Take what needs the fewer columns of products on the busiest pair, a narrow round counting a tenth more.
+bool narrow(const Product& p, int sms) {
+  const long m = (p.rows + 255) / 256 * (p.group ? 2 : 1), pairs = sms / 2, cols = (long)p.features * (p.gated ? 2 : 1);
+  const long wide = (m * ((cols + 255) / 256) + pairs - 1) / pairs * 256;
+  const long thin = (m * ((cols + 127) / 128) + pairs - 1) / pairs * 128;
+  return thin * 11 < wide * 10;
+}
+
+template <bool X_MN, bool W_MN, bool FP8, bool GATED>
+int pick(const Product& p, cudaStream_t s) {
+  int dev = 0, sms = 0;
+  JLA_CUDA_OK(cudaGetDevice(&dev));
+  JLA_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  return narrow(p, sms) ? launch<128, X_MN, W_MN, FP8, GATED>(p, sms, s) : launch<256, X_MN, W_MN, FP8, GATED>(p, sms, s);
+}
+
+}  // namespace
+
+int product_pairs(const Product& p, cudaStream_t s) {
+  if (p.dtype == JLA_DTYPE_E4M3) return p.gated ? pick<false, false, true, true>(p, s) : pick<false, false, true, false>(p, s);
+  if (p.x_mn) return pick<true, true, false, false>(p, s);
+  if (p.w_mn) return pick<false, true, false, false>(p, s);
+  return p.gated ? pick<false, false, false, true>(p, s) : pick<false, false, false, false>(p, s);
+}
+
+}  // namespace jla

@@ -8,7 +8,8 @@ enum {
   kProfTables = 0, kProfGates, kProfL2Norm, kProfKktInv, kProfSgFwd, kProfSgBwdState, kProfSgChunkGrads,
   kProfFinalize, kProfRecFwd, kProfRecBwd, kProfKdaPrep, kProfKdaIntra, kProfKdaFwd, kProfKdaBwdState,
   kProfKdaChunkGrads, kProfCpCorrection, kProfSgGradsQ, kProfSgGradsK, kProfTokenStep, kProfRecGrads, kProfSplitFwd,
-  kProfSplitOut, kProfSplitZ, kProfSplitBwd, kProfKernels
+  kProfSplitOut, kProfSplitZ, kProfSplitBwd, kProfRmsNorm, kProfRmsNormBwd, kProfProduct, kProfFewTokens, kProfActBwd,
+  kProfKernels
 };
 
 class ProfScope {

@@ -15,6 +15,10 @@ namespace tma {
 // {64 inner elements, 1, box_rows outer rows} and 128-byte swizzle. `mid` = 1 gives a plain 2-D matrix.
 // Returns false (and sets the library error text) when the driver entry point is missing or rejects the shape.
 bool encode_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t mid, uint64_t outer, uint32_t box_rows);
+// Tensor map over a matrix of `rows` rows of `inner` elements of 1, 2 or 4 bytes, `row_stride` elements apart, with box
+// {128 bytes of a row, box_rows rows} and 128-byte swizzle. Base and row stride have to be multiples of 16 bytes.
+bool encode_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t inner, uint64_t rows, uint64_t row_stride,
+               uint32_t box_rows);
 
 // ---- device -------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
@@ -29,6 +33,22 @@ __device__ __forceinline__ void load_3d(void* smem_dst, const CUtensorMap* map, 
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::
           "r"(umma::smem_addr(smem_dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c_inner), "r"(c_mid), "r"(c_outer), "r"(umma::smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void load_2d(uint32_t smem_dst, const CUtensorMap* map, int c_inner, int c_row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
+          smem_dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c_inner), "r"(c_row), "r"(bar)
+      : "memory");
+}
+// The same by one CTA of a pair that works on one tile (cta_group::2): `bar` may be the other CTA's barrier (umma::map_rank).
+__device__ __forceinline__ void load_2d_pair(uint32_t smem_dst, const CUtensorMap* map, int c_inner, int c_row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];\n" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c_inner), "r"(c_row), "r"(bar)
       : "memory");
 }
 
@@ -60,6 +80,12 @@ __device__ __forceinline__ void store_3d(const CUtensorMap* map, const void* sme
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
                "r"(umma::smem_addr(smem_src)), "r"(c_inner), "r"(c_mid), "r"(c_outer)
+               : "memory");
+}
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, uint32_t smem_src, int c_inner, int c_row) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_src), "r"(c_inner), "r"(c_row)
                : "memory");
 }
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }

@@ -61,6 +61,14 @@ def cast(x, dtype, device=None):
     return x.to(device=device, dtype=dtype).contiguous()
 
 
+def aligned(x):
+    """``x`` contiguous and on a 16-byte boundary (a slice of another tensor may start anywhere); None stays None."""
+    if x is None:
+        return None
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
 VALUE_BLOCK = 128  # value channels per head of the chunk kernels
 
 
