@@ -62,18 +62,22 @@ __global__ void __launch_bounds__(kColLanes * kRowLanes) activation_bwd_kernel(A
       float u[8], du[8];
       load8(p.z + at, z);
       load8(p.u + at, u);
+      with_activation(p.act, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        du[i] = dy[i] * activate(p.act, z[i]);
-        dy[i] *= u[i] * activation_slope(p.act, z[i]);
-      }
+        for (int i = 0; i < 8; ++i) {
+          du[i] = dy[i] * activate<act()>(z[i]);
+          dy[i] *= u[i] * activation_slope<act()>(z[i]);
+        }
+      });
       store8(static_cast<T*>(p.du) + at, du);
       store8(static_cast<T*>(p.dz) + at, dy);
     } else {
       if (p.z) {
         load8(p.z + at, z);
+        with_activation(p.act, [&](auto act) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dy[i] *= activation_slope(p.act, z[i]);
+          for (int i = 0; i < 8; ++i) dy[i] *= activation_slope<act()>(z[i]);
+        });
         store8(static_cast<T*>(p.dz) + at, dy);
       }
 #pragma unroll

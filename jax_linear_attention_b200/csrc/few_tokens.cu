@@ -7,8 +7,6 @@
 // cluster; each CTA leaves its partial sums in shared memory, and the cluster's CTAs share out the tokens among
 // themselves and add the parts up over distributed shared memory, in the order of the parts, every time the same.
 //
-// A thread of the epilogue holds one feature, so a warp's stores of one token are 32 neighbouring elements.
-//
 // Every wait is bounded, as in product_tc.cu (kStatusFewTokens).
 #include "product.cuh"
 #include "profile.cuh"
@@ -21,6 +19,7 @@ using umma::smem_addr;
 
 constexpr int kThreads = 192;  // warps 0 .. 3 epilogue, 4 loads, 5 products
 constexpr int kMaxSplit = 8;
+constexpr int kBatch = 2;  // tokens of a warp whose parts are on their way at one time
 
 struct Maps {
   CUtensorMap x[2], w[2];
@@ -52,29 +51,38 @@ template <int BN, bool GATED> struct Shape {
   static constexpr int kCols = kNeed <= 32 ? 32 : kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : 256;
 };
 
-// What is left of a feature's value at one token after the products: scales, bias, activation, residual, store.
+struct Quad {
+  float v[4];
+};
+__device__ __forceinline__ Quad quad(const float* p) {
+  if (!p) return Quad{};
+  const float4 f = __ldg(reinterpret_cast<const float4*>(p));
+  return Quad{{f.x, f.y, f.z, f.w}};
+}
+
+// What is left of four neighbouring features at one token after the products: scales, bias, activation, residual, store.
 template <bool FP8, bool GATED>
-__device__ __forceinline__ void finish(const Params& p, int token, int f, float v, float u, float ws0, float ws1, float bias) {
+__device__ __forceinline__ void finish(const Params& p, int token, int f, Quad v, Quad u, const Quad& ws0, const Quad& ws1,
+                                       const Quad& bias, float xs, uint2 res) {
   const size_t at = (size_t)token * p.features + f;
-  if constexpr (FP8) {
-    const float xs = __ldg(p.x_scale + token);
-    v *= xs * ws0;
-    if constexpr (GATED) u *= xs * ws1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (FP8) v.v[i] *= xs * ws0.v[i];
+    if constexpr (FP8 && GATED) u.v[i] *= xs * ws1.v[i];
+    if constexpr (!GATED) v.v[i] += bias.v[i];
   }
-  if constexpr (GATED) {
-    if (p.save[0]) p.save[0][at] = v, p.save[1][at] = u;
-    v = activate(p.act, v) * u;
-  } else {
-    v += bias;
-    if (p.save[0]) p.save[0][at] = v;
-    v = activate(p.act, v);
-    if (p.residual) {
-      v += p.half ? __half2float(__ldg(static_cast<const __half*>(p.residual) + at))
-                  : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.residual) + at));
-    }
+  if (p.save[0]) *reinterpret_cast<float4*>(p.save[0] + at) = make_float4(v.v[0], v.v[1], v.v[2], v.v[3]);
+  if (GATED && p.save[1]) *reinterpret_cast<float4*>(p.save[1] + at) = make_float4(u.v[0], u.v[1], u.v[2], u.v[3]);
+  with_activation(p.act, [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.v[i] = activate<act()>(v.v[i]) * (GATED ? u.v[i] : 1.f);
+  });
+  if (!GATED && p.residual) {
+    const float2 lo = unpack_out(p.half, res.x), hi = unpack_out(p.half, res.y);
+    v.v[0] += lo.x, v.v[1] += lo.y, v.v[2] += hi.x, v.v[3] += hi.y;
   }
-  if (p.half) static_cast<__half*>(p.y)[at] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at) =
+      make_uint2(pack_out(p.half, v.v[0], v.v[1]), pack_out(p.half, v.v[2], v.v[3]));
 }
 
 template <int BN, bool W_MN, bool FP8, bool GATED>
@@ -91,7 +99,28 @@ __global__ void __launch_bounds__(kThreads, 1) few_tokens_kernel(const __grid_co
   const int f0 = (int)(blockIdx.x / split) * 128, m0 = (int)blockIdx.y * BN;
   const int k_lo = (int)((long)p.kt * part / split), k_hi = (int)((long)p.kt * (part + 1) / split);
 
-  if (threadIdx.x == 0) {
+  // Step `it` of this part's contraction into its stage of the ring.
+  auto load = [&](int it) {
+    const int s = it % ST, kt = k_lo + it;
+    tma::expect_tx(full + s, S::kStageBytes);
+    const uint32_t bar = smem_addr(full + s);
+    const bool second = kt >= p.kt0;
+    const int k0 = (second ? kt - p.kt0 : kt) * (FP8 ? 128 : 64);
+    const uint32_t ws = base + s * S::kStageBytes, xs = ws + NW * S::kWeightBytes;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const CUtensorMap* mw = &maps.w[GATED ? i : (second ? 1 : 0)];
+      if constexpr (W_MN) {
+        tma::load_2d(ws + i * S::kWeightBytes, mw, f0, k0, bar);
+        tma::load_2d(ws + i * S::kWeightBytes + 8192, mw, f0 + 64, k0, bar);
+      } else {
+        tma::load_2d(ws + i * S::kWeightBytes, mw, k0, f0, bar);
+      }
+    }
+    tma::load_2d(xs, &maps.x[second ? 1 : 0], k0, m0, bar);
+  };
+  const int steps = k_hi - k_lo;
+  if (warp == 4 && lane == 0) {
     for (int i = 0; i < ST; ++i) {
       umma::mbar_init(full + i, 1);
       umma::mbar_init(empty + i, 1);
@@ -99,6 +128,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_tokens_kernel(const __grid_co
     umma::mbar_init(&done, 1);
     umma::mbar_init(&drain, 1);
     umma::mbar_init_fence();
+    umma::fence_async_smem();
+    for (int it = 0; it < ST && it < steps; ++it) load(it);  // the first copies wait for nobody
   }
   if (warp == 5) umma::tmem_alloc(&tmem_slot, S::kCols);
   umma::fence_before_sync();
@@ -108,27 +139,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_tokens_kernel(const __grid_co
   bool ok = true;
 
   if (warp == 4 && lane == 0) {
-    int it = 0;
-    for (int kt = k_lo; kt < k_hi; ++kt, ++it) {
-      const int s = it % ST;
-      if (it >= ST) ok = umma::mbar_wait(empty + s, ((it / ST) - 1) & 1);
+    int it = ST < steps ? ST : steps;
+    for (; it < steps; ++it) {
+      ok = umma::mbar_wait(empty + it % ST, ((it / ST) - 1) & 1);
       if (!ok) break;
-      tma::expect_tx(full + s, S::kStageBytes);
-      const uint32_t bar = smem_addr(full + s);
-      const bool second = kt >= p.kt0;
-      const int k0 = (second ? kt - p.kt0 : kt) * (FP8 ? 128 : 64);
-      const uint32_t ws = base + s * S::kStageBytes, xs = ws + NW * S::kWeightBytes;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        const CUtensorMap* mw = &maps.w[GATED ? i : (second ? 1 : 0)];
-        if constexpr (W_MN) {
-          tma::load_2d(ws + i * S::kWeightBytes, mw, f0, k0, bar);
-          tma::load_2d(ws + i * S::kWeightBytes + 8192, mw, f0 + 64, k0, bar);
-        } else {
-          tma::load_2d(ws + i * S::kWeightBytes, mw, k0, f0, bar);
-        }
-      }
-      tma::load_2d(xs, &maps.x[second ? 1 : 0], k0, m0, bar);
+      load(it);
     }
     if (!ok) {
       for (int j = it > ST ? it - ST : 0; j < it; ++j) umma::mbar_wait(full + j % ST, (j / ST) & 1);
@@ -137,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_tokens_kernel(const __grid_co
     const uint64_t w0 = umma::smem_desc(base, W_MN ? 8192 : 16, 1024);
     const uint64_t x0 = umma::smem_desc(base + NW * S::kWeightBytes, 16, 1024);
     int it = 0;
-    for (int kt = k_lo; kt < k_hi; ++kt, ++it) {
+    for (; it < steps; ++it) {
       const int s = it % ST;
       ok = umma::mbar_wait(full + s, (it / ST) & 1);
       if (!ok) break;
@@ -160,75 +175,79 @@ __global__ void __launch_bounds__(kThreads, 1) few_tokens_kernel(const __grid_co
       umma::mbar_wait(&drain, 0);
     }
   }
+  const int f4 = f0 + lane * 4;
+  Quad ws0{}, ws1{}, bias{};
   if (warp < 4) {
+    if (f4 < p.features) {
+      if constexpr (FP8) ws0 = quad(p.w_scale[0] + f4);
+      if constexpr (FP8 && GATED) ws1 = quad(p.w_scale[1] + f4);
+      if (!GATED && p.bias) bias = quad(p.bias + f4);
+    }
     ok = umma::mbar_wait(&done, 0);
     umma::fence_after_sync();
   }
-  const int f = f0 + warp * 32 + lane;  // (warps 0 .. 3)
-  const uint32_t acc = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+  // Partial sums [weight][token][128 features] over the ring, which is idle now. Column c of the accumulator is a token.
   const int tokens = p.rows - m0 < BN ? p.rows - m0 : BN;
-  float ws0 = 0.f, ws1 = 0.f, bias = 0.f;
-  if (warp < 4 && f < p.features) {
-    if constexpr (FP8) {
-      ws0 = __ldg(p.w_scale[0] + f);
-      if constexpr (GATED) ws1 = __ldg(p.w_scale[1] + f);
-    }
-    if (p.bias) bias = __ldg(p.bias + f);
-  }
-  constexpr int CH = BN < 32 ? BN : 32;  // columns a step (16: the last 16 of a load are not looked at)
-  if (split == 1) {
-    if (warp < 4 && __all_sync(0xffffffffu, ok)) {
+  if (warp < 4 && __all_sync(0xffffffffu, ok)) {
+    const uint32_t acc = tmem + ((uint32_t)(32 * warp) << 16);
+    constexpr int CH = BN < 32 ? BN : 32;  // (of a load of 32 columns where there are 16, the last 16 are not looked at)
 #pragma unroll 1
-      for (int c = 0; c < tokens; c += CH) {
-        float v[32], u[32];
-        umma::ld_32x32b_x32(v, acc + c);
-        if constexpr (GATED) umma::ld_32x32b_x32(u, acc + BN + c);
+    for (int c = 0; c < tokens; c += CH) {
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        float v[32];
+        umma::ld_32x32b_x32(v, acc + i * BN + c);
         umma::wait_ld();
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          if (c + i < tokens && f < p.features) finish<FP8, GATED>(p, m0 + c + i, f, v[i], GATED ? u[i] : 0.f, ws0, ws1, bias);
-        }
-      }
-    }
-  } else {
-    // partial sums [weight][token][128 features] over the ring, which is idle now
-    if (warp < 4 && __all_sync(0xffffffffu, ok)) {
-#pragma unroll 1
-      for (int c = 0; c < tokens; c += CH) {
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-          float v[32];
-          umma::ld_32x32b_x32(v, acc + i * BN + c);
-          umma::wait_ld();
-#pragma unroll
-          for (int j = 0; j < CH; ++j) {
-            if (c + j < tokens) {
-              asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(base + ((i * BN + c + j) * 128 + warp * 32 + lane) * 4), "f"(v[j])
-                           : "memory");
-            }
+        for (int j = 0; j < CH; ++j) {
+          if (c + j < tokens) {
+            asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(base + ((i * BN + c + j) * 128 + threadIdx.x) * 4), "f"(v[j])
+                         : "memory");
           }
         }
       }
     }
-    __syncwarp();
-    umma::cluster_sync();
-    if (warp < 4 && f < p.features) {
-      for (int c = part; c < tokens; c += split) {
-        float sum[NW];
+  }
+  umma::cluster_sync();
+  // The cluster's CTAs share out the tokens; a thread adds up four features of one token, a warp a whole token.
+  if (warp < 4 && f4 < p.features) {
+#pragma unroll 1
+    for (int c0 = part + warp * split; c0 < tokens; c0 += 4 * split * kBatch) {
+      Quad sum[kBatch][NW];
+#pragma unroll
+      for (int t = 0; t < kBatch; ++t) {
+        const int c = c0 + 4 * split * t;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-          const uint32_t at = base + ((i * BN + c) * 128 + warp * 32 + lane) * 4;
-          float v[kMaxSplit];
+          const uint32_t at = base + ((i * BN + c) * 128 + lane * 4) * 4;
+          Quad v[kMaxSplit];
 #pragma unroll
-          for (int r = 0; r < kMaxSplit; ++r) v[r] = r < split ? umma::ld_cluster(umma::map_rank(at, r)) : 0.f;
-          sum[i] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+          for (int r = 0; r < kMaxSplit; ++r) {
+            if (r < split && c < tokens) umma::ld_cluster4(v[r].v, umma::map_rank(at, r));
+            else v[r] = Quad{};
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sum[t][i].v[j] = ((v[0].v[j] + v[1].v[j]) + (v[2].v[j] + v[3].v[j])) + ((v[4].v[j] + v[5].v[j]) + (v[6].v[j] + v[7].v[j]));
+          }
         }
-        finish<FP8, GATED>(p, m0 + c, f, sum[0], GATED ? sum[NW - 1] : 0.f, ws0, ws1, bias);
+      }
+#pragma unroll
+      for (int t = 0; t < kBatch; ++t) {
+        const int c = c0 + 4 * split * t, token = m0 + c;
+        if (c < tokens) {
+          float xs = 1.f;
+          if constexpr (FP8) xs = __ldg(p.x_scale + token);
+          uint2 res = make_uint2(0, 0);
+          if (!GATED && p.residual) {
+            res = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + (size_t)token * p.features + f4));
+          }
+          finish<FP8, GATED>(p, token, f4, sum[t][0], sum[t][NW - 1], ws0, ws1, bias, xs, res);
+        }
       }
     }
-    __syncwarp();
-    umma::cluster_sync();  // the others read this CTA's part until here
   }
+  umma::cluster_sync();  // the others read this CTA's part until here
   if (!ok) atomicExch(p.status, kStatusFewTokens);
   umma::fence_before_sync();
   __syncthreads();
@@ -243,17 +262,16 @@ int parts(int tiles, int kt, int sms) {
 }
 
 template <int BN, bool W_MN, bool FP8, bool GATED>
-int launch(const Product& p, int sms, cudaStream_t s) {
+int launch(const Product& p, int device, int sms, cudaStream_t s) {
   using S = Shape<BN, GATED>;
   Maps maps;
   Params q{};
   const int esz = FP8 ? 1 : 2, kb = FP8 ? 128 : 64;
   bool ok = true;
   for (int i = 0; i < 2 && ok; ++i) {
-    const void *x = p.x[i] ? p.x[i] : p.x[0], *w = p.w[i] ? p.w[i] : p.w[0];
-    ok = tma::encode_2d(&maps.x[i], x, esz, p.depth, p.rows, p.x_stride, BN) &&
-         (W_MN ? tma::encode_2d(&maps.w[i], w, esz, p.features, p.depth, p.w_stride, 64)
-               : tma::encode_2d(&maps.w[i], w, esz, p.depth, p.features, p.w_stride, 128));
+    ok = (!p.x[i] || tma::encode_2d(&maps.x[i], p.x[i], esz, p.depth, p.rows, p.x_stride, BN)) &&
+         (!p.w[i] || (W_MN ? tma::encode_2d(&maps.w[i], p.w[i], esz, p.features, p.depth, p.w_stride, 64)
+                           : tma::encode_2d(&maps.w[i], p.w[i], esz, p.depth, p.features, p.w_stride, 128)));
   }
   if (!ok) return JLA_ERR_CUDA;
   q.rows = (int)p.rows, q.features = p.features;
@@ -271,7 +289,8 @@ int launch(const Product& p, int sms, cudaStream_t s) {
   const int tiles_f = (p.features + 127) / 128, tiles_m = (int)((p.rows + BN - 1) / BN);
   int split = parts(tiles_f * tiles_m, q.kt, sms);
   auto* kern = few_tokens_kernel<BN, W_MN, FP8, GATED>;
-  JLA_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  static std::atomic<uint64_t> allowed{0};
+  JLA_CUDA_OK(allow_smem(kern, S::kSmem, device, allowed));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tiles_f * split, tiles_m), cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = S::kSmem, cfg.stream = s;
@@ -290,12 +309,11 @@ int launch(const Product& p, int sms, cudaStream_t s) {
 template <bool W_MN, bool FP8, bool GATED>
 int pick(const Product& p, cudaStream_t s) {
   int dev = 0, sms = 0;
-  JLA_CUDA_OK(cudaGetDevice(&dev));
-  JLA_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  if (p.rows <= 16) return launch<16, W_MN, FP8, GATED>(p, sms, s);
-  if (p.rows <= 32) return launch<32, W_MN, FP8, GATED>(p, sms, s);
-  if (p.rows <= 64) return launch<64, W_MN, FP8, GATED>(p, sms, s);
-  return launch<128, W_MN, FP8, GATED>(p, sms, s);
+  if (const int rc = current_device(&dev, &sms)) return rc;
+  if (p.rows <= 16) return launch<16, W_MN, FP8, GATED>(p, dev, sms, s);
+  if (p.rows <= 32) return launch<32, W_MN, FP8, GATED>(p, dev, sms, s);
+  if (p.rows <= 64) return launch<64, W_MN, FP8, GATED>(p, dev, sms, s);
+  return launch<128, W_MN, FP8, GATED>(p, dev, sms, s);
 }
 
 }  // namespace

@@ -3,6 +3,9 @@
 //   linear:  z = (x W^T) xs ws + bias,  y = act(z) + residual          gated:  h = act(x Wg^T xs gs) * (x Wu^T xs us)
 #pragma once
 
+#include <atomic>
+#include <type_traits>
+
 #include "common.cuh"
 #include "tma.cuh"
 
@@ -17,20 +20,32 @@ __device__ __forceinline__ float sigmoid_f32(float z) { return fast_rcp(1.f + fa
 // gelu in its tanh form: 0.5 z (1 + tanh(t)) = z sigmoid(2 t), t = sqrt(2 / pi) (z + 0.044715 z^3)
 constexpr float kGelu2C = 1.5957691216057308f, kGeluA = 0.044715f;
 
-__device__ __forceinline__ float activate(int act, float z) {
-  if (act == kActNone) return z;
-  const float s = sigmoid_f32(act == kActGelu ? kGelu2C * (z + kGeluA * z * z * z) : z);
-  return act == kActSigmoid ? s : z * s;
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (ACT == kActNone) return z;
+  const float s = sigmoid_f32(ACT == kActGelu ? kGelu2C * (z + kGeluA * z * z * z) : z);
+  return ACT == kActSigmoid ? s : z * s;
+}
+// f(std::integral_constant) with the activation as a compile-time constant: one branch for many values
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+  switch (act) {
+    case kActSilu: f(std::integral_constant<int, kActSilu>{}); break;
+    case kActGelu: f(std::integral_constant<int, kActGelu>{}); break;
+    case kActSigmoid: f(std::integral_constant<int, kActSigmoid>{}); break;
+    default: f(std::integral_constant<int, kActNone>{}); break;
+  }
 }
 // act'(z)
-__device__ __forceinline__ float activation_slope(int act, float z) {
-  if (act == kActNone) return 1.f;
-  if (act == kActGelu) {
+template <int ACT>
+__device__ __forceinline__ float activation_slope(float z) {
+  if constexpr (ACT == kActNone) return 1.f;
+  if constexpr (ACT == kActGelu) {
     const float s = sigmoid_f32(kGelu2C * (z + kGeluA * z * z * z));
     return s + z * s * (1.f - s) * kGelu2C * (1.f + 3.f * kGeluA * z * z);
   }
   const float s = sigmoid_f32(z);
-  return act == kActSigmoid ? s * (1.f - s) : s * (1.f + z * (1.f - s));
+  return ACT == kActSigmoid ? s * (1.f - s) : s * (1.f + z * (1.f - s));
 }
 
 // Two float32 values rounded to bf16 or f16 (`half`) in one register.
@@ -76,5 +91,18 @@ int product_few_tokens(const Product& p, cudaStream_t stream);  // few_tokens.cu
 bool few_tokens_applies(const Product& p);
 
 int* tc_status_ptr();  // status.cu
+
+// The current device and its number of SMs; a jla_status.
+int current_device(int* device, int* sms);  // product_api.cu
+
+// Allows `kern` its dynamic shared memory, once on each device: `done` (one bit a device) belongs to this kernel alone.
+template <typename K>
+inline cudaError_t allow_smem(K* kern, int bytes, int device, std::atomic<uint64_t>& done) {
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 }  // namespace jla

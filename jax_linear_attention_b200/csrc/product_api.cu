@@ -4,6 +4,19 @@
 #include "product.cuh"
 
 namespace jla {
+
+int current_device(int* device, int* sms) {
+  static std::atomic<int> known[64];  // a device's SMs, 0 while nobody has asked
+  JLA_CUDA_OK(cudaGetDevice(device));
+  const bool kept = *device >= 0 && *device < 64;
+  *sms = kept ? known[*device].load(std::memory_order_relaxed) : 0;
+  if (*sms == 0) {
+    JLA_CUDA_OK(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *device));
+    if (kept) known[*device].store(*sms, std::memory_order_relaxed);
+  }
+  return JLA_OK;
+}
+
 namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -103,16 +103,17 @@ struct Staging {
   }
 };
 
-// v[i] = v[i] * s * scale[col + i], for the columns inside the matrix (a multiple of 8: whole float4s)
-__device__ __forceinline__ void scale_columns(float (&v)[32], float s, const float* scale, int col, int cols) {
+// A float for each of 64 columns from `col` on, two a lane (columns lane and 32 + lane): read before they are needed, handed
+// to all lanes by shuffles. (Every lane reading all columns' values when it needs them left the epilogue waiting on them
+// for three quarters of a tile's time.)
+struct Columns {
+  float v[2];
+  __device__ __forceinline__ void read(const float* p, int col, int lane, int cols) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
-    if (col + i < cols) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(scale + col + i));
-      v[i] *= s * f.x, v[i + 1] *= s * f.y, v[i + 2] *= s * f.z, v[i + 3] *= s * f.w;
-    }
+    for (int h = 0; h < 2; ++h) v[h] = p && col + 32 * h + lane < cols ? __ldg(p + col + 32 * h + lane) : 0.f;
   }
-}
+  __device__ __forceinline__ float at(int h, int i) const { return __shfl_sync(0xffffffffu, v[h], i); }
+};
 
 template <int BN, bool X_MN, bool W_MN, bool FP8, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -147,72 +148,85 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
   const uint32_t tmem = tmem_slot;
   bool ok = true;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // ---- loads: this CTA's 128 rows of x and its half of the weight's; the bytes count on the leader's barrier
-    tma::prefetch_map(&maps.x[0]);
-    tma::prefetch_map(&maps.w[0]);
-    int it = 0;
+    if (lane == 0) {
+      tma::prefetch_map(&maps.x[0]);
+      tma::prefetch_map(&maps.w[0]);
+    }
+    const uint32_t bars = umma::map_rank(smem_addr(full), 0), mine = smem_addr(full), freed = smem_addr(empty);
+    int s = 0, issued = 0;
+    uint32_t phase = 1;  // (a fresh barrier's phase before the first counts as complete)
     for (int t = first; t < p.tiles && ok; t += step) {
       const int g = t / p.tiles_mn;
       int tm, tn;
       locate(p, t - g * p.tiles_mn, tm, tn);
       const int m0 = tm * 256 + (int)rank * 128;
       const int n0 = GATED ? tn * (BN / 2) : tn * BN + (int)rank * (BN / 2);
-      for (int kt = 0; kt < p.kt && ok; ++kt, ++it) {
-        const int s = it % ST;
-        if (it >= ST) ok = umma::mbar_wait(empty + s, ((it / ST) - 1) & 1);
+      const CUtensorMap* mx = &maps.x[g];
+      const CUtensorMap* mw = &maps.w[GATED ? rank : 0];
+      int k0 = 0;
+      for (int kt = 0; kt < p.kt; ++kt, k0 += FP8 ? 128 : 64) {
+        if (kt == p.kt0) mx = &maps.x[1], mw = &maps.w[1], k0 = 0;  // the second pair of operands
+        ok = umma::mbar_wait_warp(freed + 8 * s, phase);
         if (!ok) break;
-        if (rank == 0) tma::expect_tx(full + s, 2 * S::kStageBytes);
-        const uint32_t bar = umma::map_rank(smem_addr(full + s), 0);
-        const bool second = kt >= p.kt0;
-        const CUtensorMap* mx = &maps.x[second ? 1 : g];
-        const CUtensorMap* mw = &maps.w[GATED ? rank : (second ? 1 : 0)];
-        const int k0 = (second ? kt - p.kt0 : kt) * (FP8 ? 128 : 64);
-        const uint32_t xs = base + s * S::kStageBytes, ws = xs + 128 * 128;
-        if constexpr (X_MN) {
-          tma::load_2d_pair(xs, mx, m0, k0, bar);
-          tma::load_2d_pair(xs + 8192, mx, m0 + 64, k0, bar);
-        } else {
-          tma::load_2d_pair(xs, mx, k0, m0, bar);
-        }
-        if constexpr (W_MN) {
+        if (umma::elect_one()) {
+          if (rank == 0) tma::expect_tx(mine + 8 * s, 2 * S::kStageBytes);
+          const uint32_t bar = bars + 8 * s, xs = base + s * S::kStageBytes, ws = xs + 128 * 128;
+          if constexpr (X_MN) {
+            tma::load_2d_pair(xs, mx, m0, k0, bar);
+            tma::load_2d_pair(xs + 8192, mx, m0 + 64, k0, bar);
+          } else {
+            tma::load_2d_pair(xs, mx, k0, m0, bar);
+          }
+          if constexpr (W_MN) {
 #pragma unroll
-          for (int b = 0; b < BN / 128; ++b) tma::load_2d_pair(ws + b * 8192, mw, n0 + b * 64, k0, bar);
-        } else {
-          tma::load_2d_pair(ws, mw, k0, n0, bar);
+            for (int b = 0; b < BN / 128; ++b) tma::load_2d_pair(ws + b * 8192, mw, n0 + b * 64, k0, bar);
+          } else {
+            tma::load_2d_pair(ws, mw, k0, n0, bar);
+          }
         }
+        __syncwarp();
+        ++issued;
+        if (++s == ST) s = 0, phase ^= 1;
       }
     }
     if (!ok && rank == 0) {  // let what was asked for land before the block's memory is given up
-      for (int j = it > ST ? it - ST : 0; j < it; ++j) umma::mbar_wait(full + j % ST, (j / ST) & 1);
+      for (int j = issued > ST ? issued - ST : 0; j < issued; ++j) umma::mbar_wait_warp(mine + 8 * (j % ST), (j / ST) & 1);
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     // ---- products
     const uint64_t x0 = umma::smem_desc(base, X_MN ? 8192 : 16, 1024);
     const uint64_t w0 = umma::smem_desc(base + 128 * 128, W_MN ? 8192 : 16, 1024);
-    int it = 0, n = 0;
+    const uint32_t filled = smem_addr(full), acc_freed = smem_addr(acc_empty);
+    int s = 0, n = 0;
+    uint32_t phase = 0;
     for (int t = first; t < p.tiles && ok; t += step, ++n) {
       const int a = n & 1;
-      if (n >= 2) ok = umma::mbar_wait(acc_empty + a, ((n >> 1) - 1) & 1);
+      ok = umma::mbar_wait_warp(acc_freed + 8 * a, ((n >> 1) & 1) ^ 1);
       umma::fence_after_sync();
-      for (int kt = 0; kt < p.kt && ok; ++kt, ++it) {
-        const int s = it % ST;
-        ok = umma::mbar_wait(full + s, (it / ST) & 1);
+      for (int kt = 0; kt < p.kt && ok; ++kt) {
+        ok = umma::mbar_wait_warp(filled + 8 * s, phase);
         if (!ok) break;
         umma::fence_after_sync();
-        const uint32_t off = (uint32_t)(s * S::kStageBytes) >> 4;
+        if (umma::elect_one()) {
+          const uint32_t off = (uint32_t)(s * S::kStageBytes) >> 4;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          umma::mma_pair<FP8>(tmem + a * BN, x0 + off + (X_MN ? ks * 128 : ks * 2), w0 + off + (W_MN ? ks * 128 : ks * 2),
-                              p.idesc, kt > 0 || ks > 0);
+          for (int ks = 0; ks < 4; ++ks) {
+            umma::mma_pair<FP8>(tmem + a * BN, x0 + off + (X_MN ? ks * 128 : ks * 2), w0 + off + (W_MN ? ks * 128 : ks * 2),
+                                p.idesc, kt > 0 || ks > 0);
+          }
+          umma::commit_pair(empty + s);
+          if (kt == p.kt - 1) umma::commit_pair(acc_full + a);
         }
-        umma::commit_pair(empty + s);
+        __syncwarp();
+        if (++s == ST) s = 0, phase ^= 1;
       }
-      if (ok) umma::commit_pair(acc_full + a);
     }
     if (!ok) {  // products in flight read both CTAs' shared memory: wait for them
-      umma::commit_pair(&drain);
-      umma::mbar_wait(&drain, 0);
+      if (umma::elect_one()) umma::commit_pair(&drain);
+      __syncwarp();
+      umma::mbar_wait_warp(smem_addr(&drain), 0);
     }
   } else if (warp >= 4) {
     // ---- epilogue: warp w owns the TMEM lanes (rows) 32 w .. 32 w + 31 of its CTA
@@ -222,32 +236,41 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     int n = 0;
     for (int t = first; t < p.tiles; t += step, ++n) {
       const int a = n & 1;
-      ok = umma::mbar_wait(acc_full + a, (n >> 1) & 1);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
-      umma::fence_after_sync();
       const int g = t / p.tiles_mn;
       int tm, tn;
       locate(p, t - g * p.tiles_mn, tm, tn);
       const int row0 = tm * 256 + (int)rank * 128 + w * 32, row = row0 + lane;
       const bool live = row < p.rows;
       const uint32_t acc = tmem + a * BN + ((uint32_t)(32 * w) << 16);
+      constexpr int COLS = GATED ? BN / 2 : BN;
+      Columns bias, scale0, scale1;
+      auto read_columns = [&](int col) {
+        if constexpr (!GATED) bias.read(p.bias, col, lane, p.features);
+        if constexpr (FP8) scale0.read(p.w_scale[0], col, lane, p.features);
+        if constexpr (FP8 && GATED) scale1.read(p.w_scale[1], col, lane, p.features);
+      };
+      read_columns(tn * COLS);
       float xs = 1.f;
       if constexpr (FP8) xs = live ? __ldg(p.x_scale + row) : 0.f;
-      constexpr int COLS = GATED ? BN / 2 : BN;
+      ok = umma::mbar_wait(acc_full + a, (n >> 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      umma::fence_after_sync();
 #pragma unroll 1
       for (int c = 0; c < COLS; c += 64) {
         const int col = tn * COLS + c;
         if (col >= p.features || row0 >= p.rows) break;
-        uint32_t out[32];
+        const Columns b = bias, s0 = scale0, s1 = scale1;
         uint4 res[8];
         if (!GATED && p.residual) {
           const uint4* r = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + (size_t)row * p.features + col);
 #pragma unroll
           for (int j = 0; j < 8; ++j) res[j] = live && col + 8 * j < p.features ? __ldg(r + j) : make_uint4(0, 0, 0, 0);
         }
+        read_columns(c + 64 < COLS ? col + 64 : p.features);
+        uint32_t out[32];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int hc = col + 32 * h;
@@ -258,32 +281,32 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             umma::ld_32x32b_x32(u, acc + BN / 2 + c + 32 * h);
             umma::wait_ld();
             if constexpr (FP8) {
-              scale_columns(v, xs, p.w_scale[0], hc, p.features);
-              scale_columns(u, xs, p.w_scale[1], hc, p.features);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] *= xs * s0.at(h, i), u[i] *= xs * s1.at(h, i);
             }
             if (p.saves) {
               stage.save32(v, lane, &maps.save[0], hc, row0, p.features, p.rows);
               stage.save32(u, lane, &maps.save[1], hc, row0, p.features, p.rows);
             }
+            with_activation(p.act, [&](auto act) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = activate(p.act, v[i]) * u[i];
+              for (int i = 0; i < 32; ++i) v[i] = activate<act()>(v[i]) * u[i];
+            });
           } else {
             umma::wait_ld();
-            if constexpr (FP8) scale_columns(v, xs, p.w_scale[0], hc, p.features);
+            if constexpr (FP8) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] *= xs * s0.at(h, i);
+            }
             if (p.bias) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                if (hc + i < p.features) {
-                  const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + hc + i));
-                  v[i] += b.x, v[i + 1] += b.y, v[i + 2] += b.z, v[i + 3] += b.w;
-                }
-              }
+              for (int i = 0; i < 32; ++i) v[i] += b.at(h, i);
             }
             if (p.saves) stage.save32(v, lane, &maps.save[0], hc, row0, p.features, p.rows);
-            if (p.act != kActNone) {
+            with_activation(p.act, [&](auto act) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = activate(p.act, v[i]);
-            }
+              for (int i = 0; i < 32; ++i) v[i] = activate<act()>(v[i]);
+            });
             if (p.residual) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
@@ -317,21 +340,19 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
 }
 
 template <int BN, bool X_MN, bool W_MN, bool FP8, bool GATED>
-int launch(const Product& p, int sms, cudaStream_t s) {
+int launch(const Product& p, int device, int sms, cudaStream_t s) {
   using S = Shape<BN>;
   Maps maps;
   Params q{};
   const int esz = FP8 ? 1 : 2, kb = FP8 ? 128 : 64;
   const int xr = X_MN ? 64 : 128, wr = W_MN ? 64 : BN / 2;
   bool ok = true;
-  for (int i = 0; i < 2 && ok; ++i) {
-    const void *x = p.x[i] ? p.x[i] : p.x[0], *w = p.w[i] ? p.w[i] : p.w[0];
-    void *y = p.y[i] ? p.y[i] : p.y[0];
-    ok = (X_MN ? tma::encode_2d(&maps.x[i], x, esz, p.rows, p.depth, p.x_stride, xr)
-               : tma::encode_2d(&maps.x[i], x, esz, p.depth, p.rows, p.x_stride, xr)) &&
-         (W_MN ? tma::encode_2d(&maps.w[i], w, esz, p.features, p.depth, p.w_stride, wr)
-               : tma::encode_2d(&maps.w[i], w, esz, p.depth, p.features, p.w_stride, wr)) &&
-         tma::encode_2d(&maps.y[i], y, 2, p.features, p.rows, p.features, 32) &&
+  for (int i = 0; i < 2 && ok; ++i) {  // (a second operand or output that is not there is not asked for either)
+    ok = (!p.x[i] || (X_MN ? tma::encode_2d(&maps.x[i], p.x[i], esz, p.rows, p.depth, p.x_stride, xr)
+                           : tma::encode_2d(&maps.x[i], p.x[i], esz, p.depth, p.rows, p.x_stride, xr))) &&
+         (!p.w[i] || (W_MN ? tma::encode_2d(&maps.w[i], p.w[i], esz, p.features, p.depth, p.w_stride, wr)
+                           : tma::encode_2d(&maps.w[i], p.w[i], esz, p.depth, p.features, p.w_stride, wr))) &&
+         (!p.y[i] || tma::encode_2d(&maps.y[i], p.y[i], 2, p.features, p.rows, p.features, 32)) &&
          (!p.save[i] || tma::encode_2d(&maps.save[i], p.save[i], 4, p.features, p.rows, p.features, 32));
   }
   if (!ok) return JLA_ERR_CUDA;
@@ -351,7 +372,8 @@ int launch(const Product& p, int sms, cudaStream_t s) {
     return JLA_ERR_CUDA;
   }
   auto* kern = product_kernel<BN, X_MN, W_MN, FP8, GATED>;
-  JLA_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  static std::atomic<uint64_t> allowed{0};
+  JLA_CUDA_OK(allow_smem(kern, S::kSmem, device, allowed));
   const int pairs = sms / 2 < q.tiles ? sms / 2 : q.tiles;
   {
     ProfScope scope(kProfProduct, s);
@@ -362,20 +384,20 @@ int launch(const Product& p, int sms, cudaStream_t s) {
 }
 
 // 256 columns a tile keep the tensor cores busier per operand byte; 128 columns waste less where the last round of tiles is
-// short. Take what needs the fewer columns of products on the busiest pair, a narrow round counting a tenth more.
+// short. Take what needs the fewer columns of products on the busiest pair, a narrow round counting half as much again (it reads L2 faster than it can).
 bool narrow(const Product& p, int sms) {
   const long m = (p.rows + 255) / 256 * (p.group ? 2 : 1), pairs = sms / 2, cols = (long)p.features * (p.gated ? 2 : 1);
   const long wide = (m * ((cols + 255) / 256) + pairs - 1) / pairs * 256;
   const long thin = (m * ((cols + 127) / 128) + pairs - 1) / pairs * 128;
-  return thin * 11 < wide * 10;
+  return thin * 3 < wide * 2;
 }
 
 template <bool X_MN, bool W_MN, bool FP8, bool GATED>
 int pick(const Product& p, cudaStream_t s) {
   int dev = 0, sms = 0;
-  JLA_CUDA_OK(cudaGetDevice(&dev));
-  JLA_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  return narrow(p, sms) ? launch<128, X_MN, W_MN, FP8, GATED>(p, sms, s) : launch<256, X_MN, W_MN, FP8, GATED>(p, sms, s);
+  if (const int rc = current_device(&dev, &sms)) return rc;
+  return narrow(p, sms) ? launch<128, X_MN, W_MN, FP8, GATED>(p, dev, sms, s)
+                        : launch<256, X_MN, W_MN, FP8, GATED>(p, dev, sms, s);
 }
 
 }  // namespace

@@ -26,6 +26,10 @@ __device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
                : "memory");
 }
 
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+
 // One box: inner coordinate c_inner (multiple of 8 elements), mid index, outer row. The mbarrier receives the bytes.
 __device__ __forceinline__ void load_3d(void* smem_dst, const CUtensorMap* map, int c_inner, int c_mid, int c_outer,
                                         uint64_t* bar) {
