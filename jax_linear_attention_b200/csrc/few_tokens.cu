@@ -4,8 +4,8 @@
 // Bound by HBM, so the weights have to stream through as many SMs as there are. The roles of the operands are swapped: 128
 // features (rows of W) fill the 128 TMEM lanes, BN tokens are the accumulator's columns, so that few tokens waste
 // neither tensor-core rows nor shared memory. The contraction is cut into up to eight parts, one for each CTA of a
-// cluster; each CTA leaves its partial sums in shared memory, and the cluster's CTAs share out the tokens among
-// themselves and add the parts up over distributed shared memory, in the order of the parts, every time the same.
+// cluster; the cluster's CTAs share out the tokens among themselves, push each other their partial sums over distributed
+// shared memory, and add the parts up in the order of the parts, every time the same.
 //
 // Every wait is bounded, as in product_tc.cu (kStatusFewTokens).
 #include "product.cuh"
@@ -17,9 +17,8 @@ namespace {
 
 using umma::smem_addr;
 
-constexpr int kThreads = 192;  // warps 0 .. 3 epilogue, 4 loads, 5 products
+constexpr int kWarps = 8, kThreads = 32 * kWarps;  // warps 0 .. 3 accumulators, 4 loads, 5 products; all of them the last sums
 constexpr int kMaxSplit = 8;
-constexpr int kBatch = 2;  // tokens of a warp whose parts are on their way at one time
 
 struct Maps {
   CUtensorMap x[2], w[2];
@@ -38,14 +37,20 @@ struct Params {
 };
 
 template <int BN, bool GATED> struct Shape {
+  static constexpr int kWeights = GATED ? 2 : 1;
   static constexpr int kWeightBytes = 128 * 128;
-  static constexpr int kStageBytes = (GATED ? 2 : 1) * kWeightBytes + BN * 128;
-  // up to 12 stages, 200 KB at most; the partial sums lie in the same memory afterwards
-  static constexpr int kFit = 200 * 1024 / kStageBytes;
+  static constexpr int kStageBytes = kWeights * kWeightBytes + BN * 128;
+  // Partial sums that arrive: whole rounds of up to eight parts, [weight][part][token][128 features].
+  static constexpr int kPartRows = BN + kMaxSplit, kPartBytes = kWeights * kPartRows * 512;
+  // The ring of operand tiles; afterwards this CTA's own partial sums, [weight][token][128 features]. Two CTAs share an SM
+  // where the sums leave room for that: twice as many clusters fit the GPU.
+  static constexpr int kCtas = kWeights * BN <= 32 ? 2 : 1;
+  static constexpr int kRoom = (kCtas == 2 ? 110 : 224) * 1024 - 1024 - kPartBytes;
+  static constexpr int kFit = kRoom / kStageBytes;
   static constexpr int kStages = kFit < 12 ? kFit : 12;
-  static constexpr int kPartBytes = (GATED ? 2 : 1) * BN * 128 * 4;
   static constexpr int kRing = kStages * kStageBytes;
-  static constexpr int kSmem = (kRing > kPartBytes ? kRing : kPartBytes) + 1024;
+  static_assert(kStages >= 2 && kRing >= kWeights * BN * 512, "the ring has to hold the partial sums");
+  static constexpr int kSmem = kRing + kPartBytes + 1024;
   // TMEM columns: a load takes 32 from the start of an accumulator, also where the accumulator has 16
   static constexpr int kNeed = (GATED ? BN : 0) + (BN < 32 ? 32 : BN);
   static constexpr int kCols = kNeed <= 32 ? 32 : kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : 256;
@@ -61,7 +66,7 @@ __device__ __forceinline__ Quad quad(const float* p) {
 }
 
 // What is left of four neighbouring features at one token after the products: scales, bias, activation, residual, store.
-template <bool FP8, bool GATED>
+template <int ACT, bool FP8, bool GATED>
 __device__ __forceinline__ void finish(const Params& p, int token, int f, Quad v, Quad u, const Quad& ws0, const Quad& ws1,
                                        const Quad& bias, float xs, uint2 res) {
   const size_t at = (size_t)token * p.features + f;
@@ -73,10 +78,8 @@ __device__ __forceinline__ void finish(const Params& p, int token, int f, Quad v
   }
   if (p.save[0]) *reinterpret_cast<float4*>(p.save[0] + at) = make_float4(v.v[0], v.v[1], v.v[2], v.v[3]);
   if (GATED && p.save[1]) *reinterpret_cast<float4*>(p.save[1] + at) = make_float4(u.v[0], u.v[1], u.v[2], u.v[3]);
-  with_activation(p.act, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v.v[i] = activate<act()>(v.v[i]) * (GATED ? u.v[i] : 1.f);
-  });
+  for (int i = 0; i < 4; ++i) v.v[i] = activate<ACT>(v.v[i]) * (GATED ? u.v[i] : 1.f);
   if (!GATED && p.residual) {
     const float2 lo = unpack_out(p.half, res.x), hi = unpack_out(p.half, res.y);
     v.v[0] += lo.x, v.v[1] += lo.y, v.v[2] += hi.x, v.v[3] += hi.y;
@@ -86,22 +89,24 @@ __device__ __forceinline__ void finish(const Params& p, int token, int f, Quad v
 }
 
 template <int BN, bool W_MN, bool FP8, bool GATED>
-__global__ void __launch_bounds__(kThreads, 1) few_tokens_kernel(const __grid_constant__ Maps maps,
+__global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_tokens_kernel(const __grid_constant__ Maps maps,
                                                                  const __grid_constant__ Params p, int split) {
   using S = Shape<BN, GATED>;
   constexpr int ST = S::kStages, NW = GATED ? 2 : 1;
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ __align__(8) uint64_t full[ST], empty[ST], done, drain;
+  __shared__ __align__(8) uint64_t full[ST], empty[ST], done, drain, arrived;
   __shared__ uint32_t tmem_slot;
   const uint32_t base = (smem_addr(smem_dyn) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = split > 1 ? (int)umma::cluster_rank() : 0;
   const int f0 = (int)(blockIdx.x / split) * 128, m0 = (int)blockIdx.y * BN;
+  const int tokens = p.rows - m0 < BN ? p.rows - m0 : BN, per = (tokens + split - 1) / split;
+  auto per_of = [&](int r) { return min(max(tokens - r * per, 0), per); };  // tokens that CTA r finishes
   const int k_lo = (int)((long)p.kt * part / split), k_hi = (int)((long)p.kt * (part + 1) / split);
 
   // Step `it` of this part's contraction into its stage of the ring.
-  auto load = [&](int it) {
-    const int s = it % ST, kt = k_lo + it;
+  auto load = [&](int it, int s) {
+    const int kt = k_lo + it;
     tma::expect_tx(full + s, S::kStageBytes);
     const uint32_t bar = smem_addr(full + s);
     const bool second = kt >= p.kt0;
@@ -120,145 +125,188 @@ __global__ void __launch_bounds__(kThreads, 1) few_tokens_kernel(const __grid_co
     tma::load_2d(xs, &maps.x[second ? 1 : 0], k0, m0, bar);
   };
   const int steps = k_hi - k_lo;
-  if (warp == 4 && lane == 0) {
-    for (int i = 0; i < ST; ++i) {
-      umma::mbar_init(full + i, 1);
-      umma::mbar_init(empty + i, 1);
+  int asked = steps < ST ? steps : ST;
+  if (warp == 4) {
+    if (umma::elect_one()) {
+      for (int i = 0; i < ST; ++i) {
+        umma::mbar_init(full + i, 1);
+        umma::mbar_init(empty + i, 1);
+      }
+      umma::mbar_init(&done, 1);
+      umma::mbar_init(&drain, 1);
+      umma::mbar_init(&arrived, 1);
+      umma::mbar_init_fence();
+      umma::fence_async_smem();
+      tma::expect_tx(&arrived, NW * split * per_of(part) * 512);
     }
-    umma::mbar_init(&done, 1);
-    umma::mbar_init(&drain, 1);
-    umma::mbar_init_fence();
-    umma::fence_async_smem();
-    for (int it = 0; it < ST && it < steps; ++it) load(it);  // the first copies wait for nobody
+    __syncwarp();
   }
   if (warp == 5) umma::tmem_alloc(&tmem_slot, S::kCols);
   umma::fence_before_sync();
-  __syncthreads();
+  umma::cluster_arrive();  // (waited for before the first partial sums leave for another CTA)
+  if (warp == 4) {  // the first copies wait for nobody
+    asm volatile("bar.arrive 1, %0;\n" ::"n"(kThreads) : "memory");
+    if (umma::elect_one()) {
+      for (int it = 0; it < asked; ++it) load(it, it);
+    }
+    __syncwarp();
+  } else {
+    asm volatile("bar.sync 1, %0;\n" ::"n"(kThreads) : "memory");
+  }
   umma::fence_after_sync();
   const uint32_t tmem = tmem_slot;
   bool ok = true;
 
-  if (warp == 4 && lane == 0) {
-    int it = ST < steps ? ST : steps;
-    for (; it < steps; ++it) {
-      ok = umma::mbar_wait(empty + it % ST, ((it / ST) - 1) & 1);
+  if (warp == 4) {
+    int s = 0;
+    uint32_t phase = 0;
+    for (int it = ST; it < steps; ++it) {
+      ok = umma::mbar_wait_warp(smem_addr(empty) + 8 * s, phase);
       if (!ok) break;
-      load(it);
+      if (umma::elect_one()) load(it, s);
+      __syncwarp();
+      asked = it + 1;
+      if (++s == ST) s = 0, phase ^= 1;
     }
     if (!ok) {
-      for (int j = it > ST ? it - ST : 0; j < it; ++j) umma::mbar_wait(full + j % ST, (j / ST) & 1);
+      for (int j = asked > ST ? asked - ST : 0; j < asked; ++j) umma::mbar_wait_warp(smem_addr(full) + 8 * (j % ST), (j / ST) & 1);
     }
-  } else if (warp == 5 && lane == 0) {
+  } else if (warp == 5) {
     const uint64_t w0 = umma::smem_desc(base, W_MN ? 8192 : 16, 1024);
     const uint64_t x0 = umma::smem_desc(base + NW * S::kWeightBytes, 16, 1024);
-    int it = 0;
-    for (; it < steps; ++it) {
-      const int s = it % ST;
-      ok = umma::mbar_wait(full + s, (it / ST) & 1);
+    int s = 0;
+    uint32_t phase = 0;
+    for (int it = 0; it < steps; ++it) {
+      ok = umma::mbar_wait_warp(smem_addr(full) + 8 * s, phase);
       if (!ok) break;
       umma::fence_after_sync();
-      const uint32_t off = (uint32_t)(s * S::kStageBytes) >> 4;
+      if (umma::elect_one()) {
+        const uint32_t off = (uint32_t)(s * S::kStageBytes) >> 4;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) {
+        for (int i = 0; i < NW; ++i) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          umma::mma_any<FP8>(tmem + i * BN, w0 + off + i * (S::kWeightBytes >> 4) + (W_MN ? ks * 128 : ks * 2),
-                             x0 + off + ks * 2, p.idesc, it > 0 || ks > 0);
+          for (int ks = 0; ks < 4; ++ks) {
+            umma::mma_any<FP8>(tmem + i * BN, w0 + off + i * (S::kWeightBytes >> 4) + (W_MN ? ks * 128 : ks * 2),
+                               x0 + off + ks * 2, p.idesc, it > 0 || ks > 0);
+          }
         }
+        umma::commit(empty + s);
+        if (it == steps - 1) umma::commit(&done);
       }
-      umma::commit(empty + s);
+      __syncwarp();
+      if (++s == ST) s = 0, phase ^= 1;
     }
-    if (ok) {
-      umma::commit(&done);
-    } else {
-      umma::commit(&drain);
-      umma::mbar_wait(&drain, 0);
+    if (!ok) {
+      if (umma::elect_one()) umma::commit(&drain);
+      __syncwarp();
+      umma::mbar_wait_warp(smem_addr(&drain), 0);
     }
   }
   const int f4 = f0 + lane * 4;
   Quad ws0{}, ws1{}, bias{};
+  if (f4 < p.features) {
+    if constexpr (FP8) ws0 = quad(p.w_scale[0] + f4);
+    if constexpr (FP8 && GATED) ws1 = quad(p.w_scale[1] + f4);
+    if (!GATED && p.bias) bias = quad(p.bias + f4);
+  }
   if (warp < 4) {
-    if (f4 < p.features) {
-      if constexpr (FP8) ws0 = quad(p.w_scale[0] + f4);
-      if constexpr (FP8 && GATED) ws1 = quad(p.w_scale[1] + f4);
-      if (!GATED && p.bias) bias = quad(p.bias + f4);
-    }
     ok = umma::mbar_wait(&done, 0);
     umma::fence_after_sync();
   }
-  // Partial sums [weight][token][128 features] over the ring, which is idle now. Column c of the accumulator is a token.
-  const int tokens = p.rows - m0 < BN ? p.rows - m0 : BN;
+  // This part's sums, [weight][token][128 features], over the ring, which is idle now. Column c of the accumulator is a token.
   if (warp < 4 && __all_sync(0xffffffffu, ok)) {
     const uint32_t acc = tmem + ((uint32_t)(32 * warp) << 16);
     constexpr int CH = BN < 32 ? BN : 32;  // (of a load of 32 columns where there are 16, the last 16 are not looked at)
 #pragma unroll 1
     for (int c = 0; c < tokens; c += CH) {
+      float v[NW][32];
+#pragma unroll
+      for (int i = 0; i < NW; ++i) umma::ld_32x32b_x32(v[i], acc + i * BN + c);
+      umma::wait_ld();
 #pragma unroll
       for (int i = 0; i < NW; ++i) {
-        float v[32];
-        umma::ld_32x32b_x32(v, acc + i * BN + c);
-        umma::wait_ld();
+        const uint32_t to = base + ((i * BN + c) * 128 + threadIdx.x) * 4;
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          if (c + j < tokens) {
-            asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(base + ((i * BN + c + j) * 128 + threadIdx.x) * 4), "f"(v[j])
-                         : "memory");
-          }
-        }
+        for (int j = 0; j < CH; ++j) asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(to + j * 512), "f"(v[i][j]) : "memory");
       }
     }
   }
-  umma::cluster_sync();
-  // The cluster's CTAs share out the tokens; a thread adds up four features of one token, a warp a whole token.
-  if (warp < 4 && f4 < p.features) {
-#pragma unroll 1
-    for (int c0 = part + warp * split; c0 < tokens; c0 += 4 * split * kBatch) {
-      Quad sum[kBatch][NW];
-#pragma unroll
-      for (int t = 0; t < kBatch; ++t) {
-        const int c = c0 + 4 * split * t;
+  // CTA r of the cluster finishes the tokens per * r .. per * (r + 1) - 1. Everybody copies it its part of them, one copy a
+  // weight and CTA, which count on its barrier; nobody waits for an answer from afar.
+  const uint32_t parts_at = base + S::kRing;
+  umma::cluster_wait();
+  if (split > 1) {
+    umma::fence_async_smem();
+    __syncthreads();
+    if (warp == 4 && lane < split) {
+      const int to = part + lane < split ? part + lane : part + lane - split;  // everybody begins with another CTA
+      const int n = per_of(to);
+      if (n > 0) {
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-          const uint32_t at = base + ((i * BN + c) * 128 + lane * 4) * 4;
-          Quad v[kMaxSplit];
-#pragma unroll
-          for (int r = 0; r < kMaxSplit; ++r) {
-            if (r < split && c < tokens) umma::ld_cluster4(v[r].v, umma::map_rank(at, r));
-            else v[r] = Quad{};
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            sum[t][i].v[j] = ((v[0].v[j] + v[1].v[j]) + (v[2].v[j] + v[3].v[j])) + ((v[4].v[j] + v[5].v[j]) + (v[6].v[j] + v[7].v[j]));
-          }
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < kBatch; ++t) {
-        const int c = c0 + 4 * split * t, token = m0 + c;
-        if (c < tokens) {
-          float xs = 1.f;
-          if constexpr (FP8) xs = __ldg(p.x_scale + token);
-          uint2 res = make_uint2(0, 0);
-          if (!GATED && p.residual) {
-            res = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + (size_t)token * p.features + f4));
-          }
-          finish<FP8, GATED>(p, token, f4, sum[t][0], sum[t][NW - 1], ws0, ws1, bias, xs, res);
+          umma::copy_cluster(umma::map_rank(parts_at + (i * S::kPartRows + part * per) * 512, to),
+                             base + (i * BN + to * per) * 512, n * 512, umma::map_rank(smem_addr(&arrived), to));
         }
       }
     }
+    ok = umma::mbar_wait_warp(smem_addr(&arrived), 0) && ok;
+  } else {
+    __syncthreads();
   }
-  umma::cluster_sync();  // the others read this CTA's part until here
+  // A thread adds up four features of one token in the order of the parts; a warp has up to four tokens on their way.
+  const uint32_t from = (split > 1 ? parts_at : base) + lane * 16;
+  const int weight_rows = split > 1 ? S::kPartRows : BN, mine = per_of(part);
+  if (f4 < p.features) {
+    with_activation(p.act, [&](auto act) {
+      constexpr int kBatch = 4;
+#pragma unroll 1
+      for (int c0 = warp; c0 < mine; c0 += kWarps * kBatch) {
+        float xs[kBatch];
+        uint2 res[kBatch];
+        Quad sum[kBatch][NW];
+        uint32_t at[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {  // (a token too many is the last one again, and not stored)
+          const int c = min(c0 + b * kWarps, mine - 1), token = m0 + part * per + c;
+          at[b] = from + c * 512;
+          xs[b] = 1.f, res[b] = make_uint2(0, 0);
+          if constexpr (FP8) xs[b] = __ldg(p.x_scale + token);
+          if (!GATED && p.residual) {
+            res[b] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + (size_t)token * p.features + f4));
+          }
+#pragma unroll
+          for (int i = 0; i < NW; ++i) sum[b][i] = Quad{};
+        }
+#pragma unroll 1
+        for (int r = 0; r < split; ++r) {
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+              float v[4];
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                           : "r"(at[b] + i * weight_rows * 512) : "memory");
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sum[b][i].v[j] += v[j];
+            }
+            at[b] += per * 512;
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          const int c = c0 + b * kWarps;
+          if (c < mine) {
+            finish<act(), FP8, GATED>(p, m0 + part * per + c, f4, sum[b][0], sum[b][NW - 1], ws0, ws1, bias, xs[b], res[b]);
+          }
+        }
+      }
+    });
+  }
   if (!ok) atomicExch(p.status, kStatusFewTokens);
   umma::fence_before_sync();
-  __syncthreads();
+  if (split > 1) umma::cluster_sync();  // the others' copies of this CTA's sums have arrived
+  else __syncthreads();
   if (warp == 5) umma::tmem_dealloc(tmem, S::kCols);
-}
-
-// Parts of the contraction: as many as keep every SM at work, each of at least two steps.
-int parts(int tiles, int kt, int sms) {
-  int s = sms / tiles;
-  if (s > kt / 2) s = kt / 2;
-  return s < 1 ? 1 : (s > kMaxSplit ? kMaxSplit : s);
 }
 
 template <int BN, bool W_MN, bool FP8, bool GATED>
@@ -287,17 +335,36 @@ int launch(const Product& p, int device, int sms, cudaStream_t s) {
     return JLA_ERR_CUDA;
   }
   const int tiles_f = (p.features + 127) / 128, tiles_m = (int)((p.rows + BN - 1) / BN);
-  int split = parts(tiles_f * tiles_m, q.kt, sms);
   auto* kern = few_tokens_kernel<BN, W_MN, FP8, GATED>;
   static std::atomic<uint64_t> allowed{0};
   JLA_CUDA_OK(allow_smem(kern, S::kSmem, device, allowed));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(tiles_f * split, tiles_m), cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = S::kSmem, cfg.stream = s;
+  cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = split, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cfg.attrs = &attr, cfg.numAttrs = 1;
+  // Parts of the contraction: as many as there is room for at one time, each of at least two steps. (A cluster lies within
+  // one of the GPU's groups of SMs, so fewer large clusters fit than their CTAs' number says; one that had to wait for
+  // another to finish would double the time.)
+  static std::atomic<int> room[64][kMaxSplit + 1];  // clusters of a size at one time, by device
+  int split = 1;
+  for (int c = kMaxSplit; c > 1; --c) {
+    if (c * 2 > q.kt || device >= 64) continue;
+    int fit = room[device][c].load(std::memory_order_relaxed);
+    if (fit == 0) {
+      attr.val.clusterDim.x = c;
+      cfg.gridDim = dim3(c);
+      JLA_CUDA_OK(cudaOccupancyMaxActiveClusters(&fit, kern, &cfg));
+      room[device][c].store(fit > 0 ? fit : -1, std::memory_order_relaxed);
+    }
+    if (tiles_f * tiles_m <= fit && tiles_f * tiles_m * c <= sms * S::kCtas) {
+      split = c;
+      break;
+    }
+  }
+  cfg.gridDim = dim3(tiles_f * split, tiles_m);
+  attr.val.clusterDim.x = split;
   {
     ProfScope scope(kProfFewTokens, s);
     JLA_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, maps, q, split));
@@ -313,7 +380,8 @@ int pick(const Product& p, cudaStream_t s) {
   if (p.rows <= 16) return launch<16, W_MN, FP8, GATED>(p, dev, sms, s);
   if (p.rows <= 32) return launch<32, W_MN, FP8, GATED>(p, dev, sms, s);
   if (p.rows <= 64) return launch<64, W_MN, FP8, GATED>(p, dev, sms, s);
-  return launch<128, W_MN, FP8, GATED>(p, dev, sms, s);
+  if constexpr (GATED) return launch<64, W_MN, FP8, GATED>(p, dev, sms, s);  // (two weights' sums of 128 tokens fit no SM)
+  else return launch<128, W_MN, FP8, GATED>(p, dev, sms, s);
 }
 
 }  // namespace
