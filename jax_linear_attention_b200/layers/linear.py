@@ -30,22 +30,18 @@ def _ptr(t):
 
 
 def _rows(x, width: int):
-    """``x [..., width]`` as ``(matrix, elements between its rows)`` without a copy where its rows allow 16-byte loads."""
-    try:
-        x = x.view(-1, width)
-    except RuntimeError:
-        x = x.reshape(-1, width)
-    if x.shape[0] <= 1 and x.stride(1) == 1:
-        stride = width
-    else:
-        stride = x.stride(0)
-    if x.stride(1) != 1 or stride < width or stride * x.element_size() % 16 or x.data_ptr() % 16:
-        x, stride = aligned(x), width
-    return x, stride
-
-
-def _empty(rows, cols, dtype, device):
-    return torch.empty(rows, cols, dtype=dtype, device=device)
+    """``x [..., width]`` as ``(tensor, rows, elements between rows)``, without a copy where its rows allow 16-byte loads."""
+    if not x.is_contiguous():
+        try:
+            flat = x.view(-1, width)
+        except RuntimeError:
+            flat = x.contiguous()
+        else:
+            stride = flat.stride(0)
+            if flat.stride(1) == 1 and stride >= width and not (stride * x.element_size() | x.data_ptr()) & 15:
+                return flat, flat.shape[0], stride
+        x = flat
+    return aligned(x), x.numel() // width, width
 
 
 def _activation_code(name: str, activation, allowed) -> int:
@@ -86,63 +82,71 @@ def _check(name: str, x, weights, scales, x_scale, out_dtype):
     return out_dtype or torch.bfloat16
 
 
-def _linear_fwd(x, stride, weight, x_scale, weight_scale, bias, residual, act: int, out_dtype, keep_z: bool):
-    rows, depth = x.shape
-    out = weight.shape[0]
-    y = _empty(rows, out, out_dtype, x.device)
-    z = _empty(rows, out, torch.float32, x.device) if keep_z else None
-    _lib.launch("jla_linear_fwd", x.device, _DTYPES[x.dtype], _DTYPES[out_dtype], rows, depth, out, x.data_ptr(), stride,
+def _plainly_fine(x, weight, out_dtype) -> bool:
+    """Whether a call without scales has nothing that ``_check`` would object to (a decoding step spends a fifth of its host
+    time there)."""
+    dtype, shape = x.dtype, weight.shape
+    return ((dtype is torch.bfloat16 or dtype is torch.float16) and weight.dtype is dtype and len(shape) == 2 and x.is_cuda
+            and x.get_device() == weight.get_device() and x.ndim > 0 and x.shape[-1] == shape[1] and shape[0] > 0
+            and shape[1] > 0 and not (shape[0] | shape[1]) & 7 and (out_dtype is None or out_dtype is dtype))
+
+
+def _linear_fwd(x, rows, stride, shape, weight, x_scale, weight_scale, bias, residual, act: int, out_dtype, keep_z: bool):
+    device, (out, depth) = x.device, weight.shape
+    y = torch.empty(shape, dtype=out_dtype, device=device)
+    z = torch.empty(rows, out, dtype=torch.float32, device=device) if keep_z else None
+    _lib.launch("jla_linear_fwd", device, _DTYPES[x.dtype], _DTYPES[out_dtype], rows, depth, out, x.data_ptr(), stride,
                 weight.data_ptr(), _ptr(x_scale), _ptr(weight_scale), _ptr(bias), act, _ptr(residual), y.data_ptr(), _ptr(z))
     return y, z
 
 
-def _grad_input(dz, weight, dz2=None, weight2=None):
-    rows, out = dz.shape
-    dx = _empty(rows, weight.shape[1], dz.dtype, dz.device)
-    _lib.launch("jla_linear_bwd_input", dz.device, _DTYPES[dz.dtype], rows, weight.shape[1], out, dz.data_ptr(),
+def _grad_input(shape, dz, weight, dz2=None, weight2=None):
+    out, depth = weight.shape
+    dx = torch.empty(shape, dtype=weight.dtype, device=weight.device)
+    _lib.launch("jla_linear_bwd_input", weight.device, _DTYPES[weight.dtype], dx.numel() // depth, depth, out, dz.data_ptr(),
                 weight.data_ptr(), _ptr(dz2), _ptr(weight2), dx.data_ptr())
     return dx
 
 
-def _grad_weight(dz, x, stride, dz2=None):
-    rows, out = dz.shape
-    depth = x.shape[1]
-    dw = _empty(out, depth, dz.dtype, dz.device)
-    dw2 = None if dz2 is None else torch.empty_like(dw)
-    _lib.launch("jla_linear_bwd_weight", dz.device, _DTYPES[dz.dtype], rows, depth, out, dz.data_ptr(), _ptr(dz2),
+def _grad_weight(weight, dz, x, rows, stride, dz2=None):
+    out, depth = weight.shape
+    dw = torch.empty_like(weight)
+    dw2 = None if dz2 is None else torch.empty_like(weight)
+    _lib.launch("jla_linear_bwd_weight", weight.device, _DTYPES[weight.dtype], rows, depth, out, dz.data_ptr(), _ptr(dz2),
                 x.data_ptr(), stride, dw.data_ptr(), _ptr(dw2))
     return dw, dw2
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act: int):
-        rows, stride = _rows(x, weight.shape[1])
-        out_shape = (*x.shape[:-1], weight.shape[0])
-        y, z = _linear_fwd(rows, stride, weight, None, None, bias, aligned(residual), act, x.dtype, act != 0)
-        ctx.save_for_backward(rows, weight, z)
-        ctx.act, ctx.stride, ctx.x_shape = act, stride, x.shape
-        return y.view(out_shape)
+    def forward(ctx, x, weight, bias, residual, act: int, shape):
+        flat, rows, stride = _rows(x, weight.shape[1])
+        y, z = _linear_fwd(flat, rows, stride, shape, weight, None, None, bias, aligned(residual), act, x.dtype, act != 0)
+        ctx.save_for_backward(flat, weight, z)
+        ctx.cfg = act, rows, stride, x.shape
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
-        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-        rows, out = x.shape[0], weight.shape[0]
-        flat = aligned(dy.reshape(rows, out))
+        act, rows, stride, x_shape = ctx.cfg
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        flat = aligned(dy)
         dz, db = flat, None
-        if (z is not None and (need_x or need_w)) or need_b:
+        if need_b or (z is not None and (need_x or need_w)):
+            out, device = weight.shape[0], weight.device
             dz = flat if z is None else torch.empty_like(flat)
-            scratch = None
+            scratch, nbytes = None, 0
             if need_b:
-                db = torch.empty(out, dtype=torch.float32, device=x.device)
-                scratch = torch.empty(_lib.load().jla_activation_bwd_scratch_bytes(rows, out), dtype=torch.uint8, device=x.device)
-            _lib.launch("jla_activation_bwd", x.device, _DTYPES[x.dtype], rows, out, ctx.act, _ptr(z), flat.data_ptr(),
-                        None if z is None else dz.data_ptr(), _ptr(db), _ptr(scratch), 0 if scratch is None else scratch.numel())
-        dx = _grad_input(dz, weight).view(ctx.x_shape) if need_x else None
-        dw = _grad_weight(dz, x, ctx.stride)[0] if need_w else None
-        return dx, dw, db, dy if need_r else None, None
+                nbytes = _lib.load().jla_activation_bwd_scratch_bytes(rows, out)
+                db = torch.empty(out, dtype=torch.float32, device=device)
+                scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            _lib.launch("jla_activation_bwd", device, _DTYPES[weight.dtype], rows, out, act, _ptr(z), flat.data_ptr(),
+                        None if z is None else dz.data_ptr(), _ptr(db), _ptr(scratch), nbytes)
+        dx = _grad_input(x_shape, dz, weight) if need_x else None
+        dw = _grad_weight(weight, dz, x, rows, stride)[0] if need_w else None
+        return dx, dw, db, dy if need_r else None, None, None
 
 
 def linear(x, weight, bias=None, *, activation: str | None = None, residual=None, x_scale=None, weight_scale=None,
@@ -158,31 +162,34 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
     form has no gradient and is refused where one would be recorded.
     """
     act = _activation_code("linear", activation, (None, "silu", "gelu", "sigmoid"))
-    dtype = _check("linear", x, (weight,), (weight_scale,), x_scale, out_dtype)
-    out_shape = (*x.shape[:-1], weight.shape[0])
-    if bias is not None and (bias.shape != weight.shape[:1] or bias.device != x.device):
-        raise ValueError(f"linear: bias must be [{weight.shape[0]}] on {x.device}; got {tuple(bias.shape)} on {bias.device}")
-    if residual is not None and (residual.shape != out_shape or residual.dtype != dtype or residual.device != x.device):
-        raise ValueError(f"linear: residual must be {dtype} {out_shape} on {x.device}; got {residual.dtype} "
+    if x_scale is None and weight_scale is None and _plainly_fine(x, weight, out_dtype):
+        dtype = x.dtype
+    else:
+        dtype = _check("linear", x, (weight,), (weight_scale,), x_scale, out_dtype)
+    shape = (*x.shape[:-1], weight.shape[0])
+    if bias is not None:
+        if bias.shape != weight.shape[:1] or bias.device != x.device:
+            raise ValueError(f"linear: bias must be [{weight.shape[0]}] on {x.device}; got {tuple(bias.shape)} on {bias.device}")
+        bias = aligned(bias if bias.dtype is torch.float32 else bias.float())
+    if residual is not None and (residual.shape != shape or residual.dtype is not dtype or residual.device != x.device):
+        raise ValueError(f"linear: residual must be {dtype} {shape} on {x.device}; got {residual.dtype} "
                          f"{tuple(residual.shape)} on {residual.device}")
     plain = nothing_to_differentiate((x, weight, bias, residual, x_scale, weight_scale))
-    if x.dtype == _E4M3 and not plain:
-        raise ValueError("linear: e4m3 operands have no gradient: call it under torch.no_grad()")
     weight = aligned(weight)
-    bias = None if bias is None else aligned(bias.float())
-    if not plain:
-        return _Linear.apply(x, weight, bias, residual, act)
-    rows, stride = _rows(x, weight.shape[1])
-    y, _ = _linear_fwd(rows, stride, weight, aligned(x_scale), aligned(weight_scale), bias, aligned(residual), act, dtype, False)
-    return y.view(out_shape)
+    if plain:
+        flat, rows, stride = _rows(x, weight.shape[1])
+        return _linear_fwd(flat, rows, stride, shape, weight, aligned(x_scale), aligned(weight_scale), bias, aligned(residual),
+                           act, dtype, False)[0]
+    if x.dtype is _E4M3:
+        raise ValueError("linear: e4m3 operands have no gradient: call it under torch.no_grad()")
+    return _Linear.apply(x, weight, bias, residual, act, shape)
 
 
-def _gated_fwd(x, stride, w_gate, w_up, x_scale, gate_scale, up_scale, act: int, out_dtype, keep: bool):
-    rows, depth = x.shape
-    out = w_gate.shape[0]
-    h = _empty(rows, out, out_dtype, x.device)
-    g, u = (_empty(rows, out, torch.float32, x.device) for _ in range(2)) if keep else (None, None)
-    _lib.launch("jla_gated_linear_fwd", x.device, _DTYPES[x.dtype], _DTYPES[out_dtype], rows, depth, out, x.data_ptr(), stride,
+def _gated_fwd(x, rows, stride, shape, w_gate, w_up, x_scale, gate_scale, up_scale, act: int, out_dtype, keep: bool):
+    device, (out, depth) = x.device, w_gate.shape
+    h = torch.empty(shape, dtype=out_dtype, device=device)
+    g, u = (torch.empty(rows, out, dtype=torch.float32, device=device) for _ in range(2)) if keep else (None, None)
+    _lib.launch("jla_gated_linear_fwd", device, _DTYPES[x.dtype], _DTYPES[out_dtype], rows, depth, out, x.data_ptr(), stride,
                 w_gate.data_ptr(), w_up.data_ptr(), _ptr(x_scale), _ptr(gate_scale), _ptr(up_scale), act, h.data_ptr(),
                 _ptr(g), _ptr(u))
     return h, g, u
@@ -190,32 +197,32 @@ def _gated_fwd(x, stride, w_gate, w_up, x_scale, gate_scale, up_scale, act: int,
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, act: int):
-        rows, stride = _rows(x, w_gate.shape[1])
-        h, g, u = _gated_fwd(rows, stride, w_gate, w_up, None, None, None, act, x.dtype, True)
-        ctx.save_for_backward(rows, w_gate, w_up, g, u)
-        ctx.act, ctx.stride, ctx.x_shape = act, stride, x.shape
-        return h.view(*x.shape[:-1], w_gate.shape[0])
+    def forward(ctx, x, w_gate, w_up, act: int, shape):
+        flat, rows, stride = _rows(x, w_gate.shape[1])
+        h, g, u = _gated_fwd(flat, rows, stride, shape, w_gate, w_up, None, None, None, act, x.dtype, True)
+        ctx.save_for_backward(flat, w_gate, w_up, g, u)
+        ctx.cfg = act, rows, stride, x.shape
+        return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         x, w_gate, w_up, g, u = ctx.saved_tensors
-        need_x, need_g, need_u, _ = ctx.needs_input_grad
-        rows, out = g.shape
-        dh = aligned(dh.reshape(rows, out))
+        act, rows, stride, x_shape = ctx.cfg
+        need_x, need_g, need_u = ctx.needs_input_grad[:3]
+        dh = aligned(dh)
         dg, du = torch.empty_like(dh), torch.empty_like(dh)
-        _lib.launch("jla_gated_activation_bwd", x.device, _DTYPES[x.dtype], rows, out, ctx.act, g.data_ptr(), u.data_ptr(),
-                    dh.data_ptr(), dg.data_ptr(), du.data_ptr())
-        dx = _grad_input(dg, w_gate, du, w_up).view(ctx.x_shape) if need_x else None
+        _lib.launch("jla_gated_activation_bwd", dh.device, _DTYPES[dh.dtype], rows, w_gate.shape[0], act, g.data_ptr(),
+                    u.data_ptr(), dh.data_ptr(), dg.data_ptr(), du.data_ptr())
+        dx = _grad_input(x_shape, dg, w_gate, du, w_up) if need_x else None
         d_gate = d_up = None
         if need_g and need_u:
-            d_gate, d_up = _grad_weight(dg, x, ctx.stride, du)
+            d_gate, d_up = _grad_weight(w_gate, dg, x, rows, stride, du)
         elif need_g:
-            d_gate = _grad_weight(dg, x, ctx.stride)[0]
+            d_gate = _grad_weight(w_gate, dg, x, rows, stride)[0]
         elif need_u:
-            d_up = _grad_weight(du, x, ctx.stride)[0]
-        return dx, d_gate, d_up, None
+            d_up = _grad_weight(w_up, du, x, rows, stride)[0]
+        return dx, d_gate, d_up, None, None
 
 
 def gated_linear(x, w_gate, w_up, *, activation: str = "silu", x_scale=None, gate_scale=None, up_scale=None, out_dtype=None):
@@ -226,13 +233,18 @@ def gated_linear(x, w_gate, w_up, *, activation: str = "silu", x_scale=None, gat
     [...]``, ``gate_scale [out]`` and ``up_scale [out]`` as in ``linear``, without gradients.
     """
     act = _activation_code("gated_linear", activation, ("silu", "gelu", "sigmoid"))
-    dtype = _check("gated_linear", x, (w_gate, w_up), (gate_scale, up_scale), x_scale, out_dtype)
+    if (x_scale is None and gate_scale is None and up_scale is None and _plainly_fine(x, w_gate, out_dtype)
+            and w_up.dtype is x.dtype and w_up.shape == w_gate.shape and w_up.device == x.device):
+        dtype = x.dtype
+    else:
+        dtype = _check("gated_linear", x, (w_gate, w_up), (gate_scale, up_scale), x_scale, out_dtype)
+    shape = (*x.shape[:-1], w_gate.shape[0])
     plain = nothing_to_differentiate((x, w_gate, w_up, x_scale, gate_scale, up_scale))
-    if x.dtype == _E4M3 and not plain:
-        raise ValueError("gated_linear: e4m3 operands have no gradient: call it under torch.no_grad()")
     w_gate, w_up = aligned(w_gate), aligned(w_up)
-    if not plain:
-        return _GatedLinear.apply(x, w_gate, w_up, act)
-    rows, stride = _rows(x, w_gate.shape[1])
-    h, _, _ = _gated_fwd(rows, stride, w_gate, w_up, aligned(x_scale), aligned(gate_scale), aligned(up_scale), act, dtype, False)
-    return h.view(*x.shape[:-1], w_gate.shape[0])
+    if plain:
+        flat, rows, stride = _rows(x, w_gate.shape[1])
+        return _gated_fwd(flat, rows, stride, shape, w_gate, w_up, aligned(x_scale), aligned(gate_scale), aligned(up_scale), act,
+                          dtype, False)[0]
+    if x.dtype is _E4M3:
+        raise ValueError("gated_linear: e4m3 operands have no gradient: call it under torch.no_grad()")
+    return _GatedLinear.apply(x, w_gate, w_up, act, shape)

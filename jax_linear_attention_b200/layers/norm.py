@@ -116,14 +116,14 @@ class _RMSNorm(torch.autograd.Function):
 
 
 def _rms_norm_fwd(x, residual, weight, eps, e4m3, keep_rstd):
-    dim = x.shape[-1]
+    dim, device = x.shape[-1], x.device
     rows = x.numel() // dim
     y = torch.empty_like(x, dtype=torch.float8_e4m3fn) if e4m3 else torch.empty_like(x)
     stream = None if residual is None else torch.empty_like(x)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if keep_rstd else None
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if e4m3 else None
-    _lib.launch("jla_rms_norm_fwd", x.device, _DTYPES[x.dtype], rows, dim, x.data_ptr(),
-                None if residual is None else residual.data_ptr(), weight.data_ptr(), eps, int(e4m3), y.data_ptr(),
+    rstd = torch.empty(rows, dtype=torch.float32, device=device) if keep_rstd else None
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=device) if e4m3 else None
+    _lib.launch("jla_rms_norm_fwd", device, _DTYPES[x.dtype], rows, dim, x.data_ptr(),
+                None if residual is None else residual.data_ptr(), weight.data_ptr(), eps, e4m3, y.data_ptr(),
                 None if stream is None else stream.data_ptr(), None if rstd is None else rstd.data_ptr(),
                 None if scale is None else scale.data_ptr())
     return y, stream, rstd, scale
@@ -155,7 +155,7 @@ def rms_norm(x, weight, *, residual=None, eps: float = 1e-6, out_dtype=None):
     plain = nothing_to_differentiate((x, weight, residual))
     if e4m3 and not plain:
         raise ValueError("an e4m3 output has no gradient: call rms_norm under torch.no_grad(), or with out_dtype=None")
-    x, weight, residual = aligned(x), aligned(weight.float()), aligned(residual)
+    x, weight, residual = aligned(x), aligned(weight if weight.dtype is torch.float32 else weight.float()), aligned(residual)
     if plain:
         y, stream, _, scale = _rms_norm_fwd(x, residual, weight, float(eps), e4m3, False)
     else:

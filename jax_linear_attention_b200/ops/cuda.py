@@ -63,10 +63,10 @@ def cast(x, dtype, device=None):
 
 def aligned(x):
     """``x`` contiguous and on a 16-byte boundary (a slice of another tensor may start anywhere); None stays None."""
-    if x is None:
-        return None
+    if x is None or (x.is_contiguous() and not x.data_ptr() & 15):
+        return x
     x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
+    return x.clone() if x.data_ptr() & 15 else x
 
 
 VALUE_BLOCK = 128  # value channels per head of the chunk kernels
