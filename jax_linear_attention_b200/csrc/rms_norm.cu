@@ -10,15 +10,17 @@
 //   dx = dstream + rstd (dy weight - n mean(dy weight n)),  dweight = sum over rows of dy n
 //
 // Bound by HBM. The row lies in registers between its two uses (the norm, then the values), so every tensor is read and
-// written once. A row belongs to a group of threads, a power of two, each with VPT vectors of VEC adjacent channels: 8
-// channels in 16-byte loads where the width and the addresses allow it, else single channels (neighbouring threads still
-// read neighbouring channels). Sums are held in float32. The norm is taken of the unrounded t, and the backward pass adds x
+// written once. A row belongs to a group of threads, a power of two, each with VPT vectors of VEC adjacent channels: 16
+// bytes where the width and the addresses allow it, else single channels (neighbouring threads still read neighbouring
+// channels). Sums are held in float32. The norm is taken of the unrounded t, and the backward pass adds x
 // and the residual up again: the rounded stream, half the bytes to read, would leave the float32 weight gradient with an
 // error of 2e-3 instead of 2e-7.
 //
 // The weight gradient is summed in registers over the rows that a thread walks, over the block in shared memory, and
 // over the blocks by column_sums(), always in the same order.
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 #include "column_sums.cuh"
 #include "profile.cuh"
@@ -43,38 +45,125 @@ struct RmsParams {
   float* partial;  // [gridDim.x][dim], or NULL where no weight gradient is wanted
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float (&f)[VEC]) {
-  if constexpr (VEC == 1) {
-    f[0] = to_f32(*p);
-  } else if constexpr (sizeof(T) == 2) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&u);
+// VEC adjacent elements of T as they lie in memory (16 bytes, or one element), and as floats in pairs.
+template <typename T, int VEC> struct Raw {
+  typedef typename std::conditional<VEC == 1, T, uint4>::type Bits;
+  static_assert(VEC == 1 || VEC * sizeof(T) == 16, "a vector is 16 bytes");
+  Bits bits;
+  __device__ __forceinline__ void load(const T* p) { bits = *reinterpret_cast<const Bits*>(p); }
+  __device__ __forceinline__ void zero() {
+    if constexpr (VEC == 1) bits = from_f32<T>(0.f);
+    else bits = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void get(float (&f)[VEC]) const {
+    if constexpr (VEC == 1) {
+      f[0] = to_f32(bits);
+    } else {
+      const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = to_f32(e[i]);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, float>::value) {
+          f[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          f[2 * i] = v.x, f[2 * i + 1] = v.y;
+        } else {
+          f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
+    if constexpr (VEC == 1) {
+      *p = from_f32<T>(f[0]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, float>::value) {
+          w[i] = __float_as_uint(f[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+};
+
+template <int VEC>
+__device__ __forceinline__ void load_weight(const float* p, float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    f[0] = __ldg(p);
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; i += 4) {
-      const float4 u = *reinterpret_cast<const float4*>(p + i);
+      const float4 u = __ldg(reinterpret_cast<const float4*>(p + i));
       f[i] = u.x, f[i + 1] = u.y, f[i + 2] = u.z, f[i + 3] = u.w;
     }
   }
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
+// Products and sums of VEC floats, two an instruction where there are two.
+template <int VEC>
+__device__ __forceinline__ void add_to(float (&a)[VEC], const float (&b)[VEC]) {
   if constexpr (VEC == 1) {
-    *p = from_f32<T>(f[0]);
-  } else if constexpr (sizeof(T) == 2) {
-    uint4 u;
-    T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(f[i]);
-    *reinterpret_cast<uint4*>(p) = u;
+    a[0] += b[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    for (int i = 0; i < VEC; i += 2) {
+      const float2 v = unpack2f(add2(pack2f(a[i], a[i + 1]), pack2f(b[i], b[i + 1])));
+      a[i] = v.x, a[i + 1] = v.y;
+    }
   }
+}
+template <int VEC>
+__device__ __forceinline__ void scale_by(float (&a)[VEC], float s) {
+  if constexpr (VEC == 1) {
+    a[0] *= s;
+  } else {
+    const f32x2 ss = pack2f(s, s);
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const float2 v = unpack2f(mul2(pack2f(a[i], a[i + 1]), ss));
+      a[i] = v.x, a[i + 1] = v.y;
+    }
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void multiply_by(float (&a)[VEC], const float (&b)[VEC]) {
+  if constexpr (VEC == 1) {
+    a[0] *= b[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const float2 v = unpack2f(mul2(pack2f(a[i], a[i + 1]), pack2f(b[i], b[i + 1])));
+      a[i] = v.x, a[i + 1] = v.y;
+    }
+  }
+}
+// acc += a b, element by element
+template <int VEC>
+__device__ __forceinline__ void fma_to(float (&acc)[VEC], const float (&a)[VEC], const float (&b)[VEC]) {
+  if constexpr (VEC == 1) {
+    acc[0] += a[0] * b[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const float2 v = unpack2f(fma2(pack2f(a[i], a[i + 1]), pack2f(b[i], b[i + 1]), pack2f(acc[i], acc[i + 1])));
+      acc[i] = v.x, acc[i + 1] = v.y;
+    }
+  }
+}
+template <int VEC>
+__device__ __forceinline__ float sum_of(const float (&a)[VEC]) {
+  if constexpr (VEC == 1) return a[0];
+  else if constexpr (VEC == 4) return (a[0] + a[1]) + (a[2] + a[3]);
+  else return ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
 }
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins: the scale of a row that holds one is NaN
@@ -107,41 +196,38 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
 template <typename T, int VEC, int VPT, bool E4M3>
 __global__ void __launch_bounds__(1024) rms_norm_fwd_kernel(RmsParams p) {
   __shared__ float red[2][32];
+  typedef Raw<T, VEC> R;
   const long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
   const bool live = row < p.rows;
   const size_t base = (size_t)(live ? row : 0) * p.dim;
   const int tpr = blockDim.x;
   const T* x = static_cast<const T*>(p.x);
   const T* res = static_cast<const T*>(p.residual);
-  float f[VPT][VEC];
-  float ss = 0.f;
+  R xr[VPT], rr[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int c = (j * tpr + threadIdx.x) * VEC;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[j][i] = 0.f;
-    if (live && c < p.dim) load_vec<T, VEC>(x + base + c, f[j]);
+    const bool on = live && c < p.dim;
+    xr[j].zero(), rr[j].zero();
+    if (on) xr[j].load(x + base + c);
+    if (on && res) rr[j].load(res + base + c);
   }
-  if (res) {
-    T* stream = static_cast<T*>(p.stream);
+  float f[VPT][VEC], sq[VEC];
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int c = (j * tpr + threadIdx.x) * VEC;
-      if (live && c < p.dim) {
-        float r[VEC];
-        load_vec<T, VEC>(res + base + c, r);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f[j][i] += r[i];
-        store_vec<T, VEC>(stream + base + c, f[j]);
-      }
-    }
-  }
+  for (int i = 0; i < VEC; ++i) sq[i] = 0.f;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) ss += f[j][i] * f[j][i];
+    xr[j].get(f[j]);
+    if (res) {
+      float r[VEC];
+      rr[j].get(r);
+      add_to<VEC>(f[j], r);
+      const int c = (j * tpr + threadIdx.x) * VEC;
+      if (live && c < p.dim) R::store(static_cast<T*>(p.stream) + base + c, f[j]);
+    }
+    fma_to<VEC>(sq, f[j], f[j]);
   }
-  const float rstd = rsqrtf(row_reduce<false>(ss, red[0]) / (float)p.dim + p.eps);
+  const float rstd = rsqrtf(row_reduce<false>(sum_of<VEC>(sq), red[0]) / (float)p.dim + p.eps);
   if (p.rstd && live && threadIdx.x == 0) p.rstd[row] = rstd;
   float top = 0.f;
 #pragma unroll
@@ -149,14 +235,14 @@ __global__ void __launch_bounds__(1024) rms_norm_fwd_kernel(RmsParams p) {
     const int c = (j * tpr + threadIdx.x) * VEC;
     if (c < p.dim) {
       float w[VEC];
-      load_vec<float, VEC>(p.w + c, w);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) f[j][i] = f[j][i] * rstd * w[i];
+      load_weight<VEC>(p.w + c, w);
+      scale_by<VEC>(f[j], rstd);
+      multiply_by<VEC>(f[j], w);
       if constexpr (E4M3) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) top = max_nan(top, fabsf(f[j][i]));
       } else if (live) {
-        store_vec<T, VEC>(static_cast<T*>(p.y) + base + c, f[j]);
+        R::store(static_cast<T*>(p.y) + base + c, f[j]);
       }
     }
   }
@@ -164,22 +250,25 @@ __global__ void __launch_bounds__(1024) rms_norm_fwd_kernel(RmsParams p) {
     float scale = row_reduce<true>(top, red[1]) / kE4m3Max;
     if (scale < 1.17549435e-38f) scale = 1.f;  // a row of zeros (or of subnormal numbers, which e4m3 then holds as zeros)
     if (live && threadIdx.x == 0) p.scale[row] = scale;
+    const float inv = 1.f / scale;  // (one division a row: a value within 2^-23 of the middle of two codes may take either)
     unsigned char* q = static_cast<unsigned char*>(p.y);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int c = (j * tpr + threadIdx.x) * VEC;
       if (live && c < p.dim) {
-        if constexpr (VEC == 8) {
-          __nv_fp8x2_storage_t e[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            e[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[j][2 * i] / scale, f[j][2 * i + 1] / scale), __NV_SATFINITE,
-                                            __NV_E4M3);
-          }
-          *reinterpret_cast<uint2*>(q + base + c) =
-              make_uint2((uint32_t)e[0] | ((uint32_t)e[1] << 16), (uint32_t)e[2] | ((uint32_t)e[3] << 16));
+        scale_by<VEC>(f[j], inv);
+        if constexpr (VEC == 1) {
+          q[base + c] = __nv_cvt_float_to_fp8(f[j][0], __NV_SATFINITE, __NV_E4M3);
         } else {
-          q[base + c] = __nv_cvt_float_to_fp8(f[j][0] / scale, __NV_SATFINITE, __NV_E4M3);
+          uint32_t e[VEC / 4];
+#pragma unroll
+          for (int i = 0; i < VEC / 4; ++i) {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[j][4 * i], f[j][4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[j][4 * i + 2], f[j][4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+            e[i] = lo | (hi << 16);
+          }
+          if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(q + base + c) = e[0];
+          else *reinterpret_cast<uint2*>(q + base + c) = make_uint2(e[0], e[1]);
         }
       }
     }
@@ -187,11 +276,15 @@ __global__ void __launch_bounds__(1024) rms_norm_fwd_kernel(RmsParams p) {
 }
 
 // Blocks walk the rows blockIdx.x * blockDim.y + threadIdx.y, + gridDim.x * blockDim.y, ... (the same number of steps for
-// all threads of a block: row_reduce may synchronise it).
+// all threads of a block: row_reduce may synchronise it). The next row's loads leave before a row is worked on: with four
+// tensors to read, the loads of one row in flight at a time left HBM at 4.1 TB/s.
+// (Blocks of 1024 threads have no registers for that.)
 template <typename T, int VEC, int VPT, int MAXT>
 __global__ void __launch_bounds__(MAXT) rms_norm_bwd_kernel(RmsParams p) {
+  constexpr bool kAhead = MAXT < 1024;
   __shared__ float red[2][32];
   extern __shared__ float fold[];  // [blockDim.y][dim] of the weight gradient, where a block has several rows
+  typedef Raw<T, VEC> R;
   const int tpr = blockDim.x;
   const T* x = static_cast<const T*>(p.x);
   const T* res = static_cast<const T*>(p.residual);
@@ -204,54 +297,68 @@ __global__ void __launch_bounds__(MAXT) rms_norm_bwd_kernel(RmsParams p) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[j][i] = 0.f;
   }
-  int turn = 0;
-  for (long r0 = (long)blockIdx.x * blockDim.y; r0 < p.rows; r0 += (long)gridDim.x * blockDim.y, turn ^= 1) {
+  R xr[VPT], rr[VPT], dr[VPT], sr[VPT];
+  float rstd_next = 0.f;
+  auto request = [&](long r0) {
     const long row = r0 + threadIdx.y;
     const bool live = row < p.rows;
     const size_t base = (size_t)(live ? row : 0) * p.dim;
-    float n[VPT][VEC], d[VPT][VEC], s[VPT][VEC];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int c = (j * tpr + threadIdx.x) * VEC;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) n[j][i] = d[j][i] = s[j][i] = 0.f;
-      if (live && c < p.dim) {
-        load_vec<T, VEC>(x + base + c, n[j]);
-        load_vec<T, VEC>(dy + base + c, d[j]);
-        if (ds) load_vec<T, VEC>(ds + base + c, s[j]);
-        if (res) {
-          float r[VEC];
-          load_vec<T, VEC>(res + base + c, r);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) n[j][i] += r[i];
-        }
+      const bool on = live && c < p.dim;
+      xr[j].zero(), rr[j].zero(), dr[j].zero(), sr[j].zero();
+      if (on) {
+        xr[j].load(x + base + c);
+        dr[j].load(dy + base + c);
+        if (res) rr[j].load(res + base + c);
+        if (ds) sr[j].load(ds + base + c);
       }
     }
-    const float rstd = live ? p.rstd[row] : 0.f;
-    float dot = 0.f;
+    rstd_next = live ? p.rstd[row] : 0.f;
+  };
+  const long first = (long)blockIdx.x * blockDim.y, step = (long)gridDim.x * blockDim.y;
+  if (kAhead && first < p.rows) request(first);
+  int turn = 0;
+  for (long r0 = first; r0 < p.rows; r0 += step, turn ^= 1) {
+    const long row = r0 + threadIdx.y;
+    const bool live = row < p.rows;
+    const size_t base = (size_t)(live ? row : 0) * p.dim;
+    if (!kAhead) request(r0);
+    const float rstd = rstd_next;
+    float n[VPT][VEC], d[VPT][VEC], s[VPT][VEC], dot[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) dot[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      xr[j].get(n[j]), dr[j].get(d[j]), sr[j].get(s[j]);
+      if (res) {
+        float r[VEC];
+        rr[j].get(r);
+        add_to<VEC>(n[j], r);
+      }
+    }
+    if (kAhead && r0 + step < p.rows) request(r0 + step);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int c = (j * tpr + threadIdx.x) * VEC;
       if (c < p.dim) {
         float w[VEC];
-        load_vec<float, VEC>(p.w + c, w);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          n[j][i] *= rstd;
-          dw[j][i] += d[j][i] * n[j][i];
-          d[j][i] *= w[i];
-          dot += d[j][i] * n[j][i];
-        }
+        load_weight<VEC>(p.w + c, w);
+        scale_by<VEC>(n[j], rstd);
+        fma_to<VEC>(dw[j], d[j], n[j]);
+        multiply_by<VEC>(d[j], w);
+        fma_to<VEC>(dot, d[j], n[j]);
       }
     }
-    const float mean = row_reduce<false>(dot, red[turn]) * inv_dim;
+    const float mean = row_reduce<false>(sum_of<VEC>(dot), red[turn]) * inv_dim;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int c = (j * tpr + threadIdx.x) * VEC;
       if (live && c < p.dim) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s[j][i] += rstd * (d[j][i] - n[j][i] * mean);
-        store_vec<T, VEC>(static_cast<T*>(p.dx) + base + c, s[j]);
+        R::store(static_cast<T*>(p.dx) + base + c, s[j]);
       }
     }
   }
@@ -261,7 +368,10 @@ __global__ void __launch_bounds__(MAXT) rms_norm_bwd_kernel(RmsParams p) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int c = (j * tpr + threadIdx.x) * VEC;
-      if (c < p.dim) store_vec<float, VEC>(fold + (size_t)threadIdx.y * p.dim + c, dw[j]);
+      if (c < p.dim) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) fold[(size_t)threadIdx.y * p.dim + c + i] = dw[j][i];
+      }
     }
     __syncthreads();
     for (int c = threadIdx.y * tpr + threadIdx.x; c < p.dim; c += tpr * blockDim.y) {
@@ -273,7 +383,10 @@ __global__ void __launch_bounds__(MAXT) rms_norm_bwd_kernel(RmsParams p) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int c = (j * tpr + threadIdx.x) * VEC;
-      if (c < p.dim) store_vec<float, VEC>(out + c, dw[j]);
+      if (c < p.dim) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[c + i] = dw[j][i];
+      }
     }
   }
 }
@@ -294,56 +407,62 @@ const char* problem(int dtype, long rows, int dim) {
   return nullptr;
 }
 
-template <typename T, bool E4M3>
-void launch_fwd(const RmsParams& p, bool vec, cudaStream_t s) {
-  // Threads of a row, and vectors of a thread. Few rows: one vector a thread, so that a row's loads all leave at once
-  // (a decoding step is latency). Many rows: four vectors, fewer threads meet in the reduction and more rows are in flight.
-  const int vectors = vec ? p.dim / 8 : p.dim;
-  int vpt = vec ? (vectors <= 1024 && p.rows <= 148 ? 1 : 4) : (vectors <= 4096 ? 4 : 16);
+// Threads of a row (a power of two), its vectors a thread, and rows a block.
+struct RowShape {
+  int tpr, vpt, rpb;
+};
+RowShape row_shape(int vectors, int vpt) {
   int tpr = ceil_pow2((vectors + vpt - 1) / vpt);
   if (tpr < 8) tpr = 8;
-  const int rpb = tpr >= 256 ? 1 : 256 / tpr;
-  const dim3 block(tpr, rpb), grid((unsigned)((p.rows + rpb - 1) / rpb));
+  return {tpr, vpt, tpr >= 256 ? 1 : 256 / tpr};
+}
+
+template <typename T, bool E4M3>
+void launch_fwd(const RmsParams& p, bool vec, cudaStream_t s) {
+  // Few rows: one vector a thread, so that a row's loads all leave at once (a decoding step is latency). Many rows: four
+  // vectors, fewer threads meet in the reduction and more rows are in flight.
+  constexpr int VEC = 16 / sizeof(T);
+  const int vectors = vec ? p.dim / VEC : p.dim;
+  const RowShape b = row_shape(vectors, vec ? (vectors <= 1024 && p.rows <= 148 ? 1 : 4) : (vectors <= 4096 ? 4 : 16));
+  const dim3 block(b.tpr, b.rpb), grid((unsigned)((p.rows + b.rpb - 1) / b.rpb));
   if (vec) {
-    if (vpt == 1) rms_norm_fwd_kernel<T, 8, 1, E4M3><<<grid, block, 0, s>>>(p);
-    else rms_norm_fwd_kernel<T, 8, 4, E4M3><<<grid, block, 0, s>>>(p);
+    if (b.vpt == 1) rms_norm_fwd_kernel<T, VEC, 1, E4M3><<<grid, block, 0, s>>>(p);
+    else rms_norm_fwd_kernel<T, VEC, 4, E4M3><<<grid, block, 0, s>>>(p);
   } else {
-    if (vpt == 4) rms_norm_fwd_kernel<T, 1, 4, E4M3><<<grid, block, 0, s>>>(p);
+    if (b.vpt == 4) rms_norm_fwd_kernel<T, 1, 4, E4M3><<<grid, block, 0, s>>>(p);
     else rms_norm_fwd_kernel<T, 1, 16, E4M3><<<grid, block, 0, s>>>(p);
   }
 }
 
-struct BwdShape {
-  int tpr, rpb, vpt, blocks;
-};
-BwdShape bwd_shape(long rows, int dim, bool vec) {
-  BwdShape b;
-  const int vectors = vec ? dim / 8 : dim;
-  b.vpt = vec ? 2 : (vectors <= 4096 ? 4 : 16);
-  b.tpr = ceil_pow2((vectors + b.vpt - 1) / b.vpt);
-  if (b.tpr < 8) b.tpr = 8;
-  b.rpb = b.tpr >= 256 ? 1 : 256 / b.tpr;
-  const long groups = (rows + b.rpb - 1) / b.rpb;
-  const long most = b.tpr > 512 ? 148 : (b.tpr > 256 ? 296 : kMaxParts);
-  b.blocks = (int)(groups < most ? groups : most);
-  return b;
+// Backward: two vectors a thread (registers), four where a block would not have the threads.
+RowShape bwd_shape(int dim, int vec) {
+  const int vectors = dim / vec;
+  return row_shape(vectors, vec > 1 ? (vectors <= 2048 ? 2 : 4) : (vectors <= 4096 ? 4 : 16));
+}
+// Blocks that walk the rows: two of 256 threads an SM are there at one time (by their registers), one of 512 or 1024.
+int bwd_blocks(long rows, const RowShape& b) {
+  const long groups = (rows + b.rpb - 1) / b.rpb, most = b.tpr > 256 ? 148 : 296;
+  return (int)(groups < most ? groups : most);
 }
 
 template <typename T>
-cudaError_t launch_bwd(const RmsParams& p, const BwdShape& b, bool vec, cudaStream_t s) {
+void launch_bwd(const RmsParams& p, const RowShape& b, int blocks, bool vec, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
   const dim3 block(b.tpr, b.rpb);
   const size_t smem = b.rpb > 1 && p.partial ? (size_t)b.rpb * p.dim * sizeof(float) : 0;  // at most 16 KB
-  const bool wide = b.tpr > 256;
-  if (vec) {
-    if (wide) rms_norm_bwd_kernel<T, 8, 2, 1024><<<b.blocks, block, smem, s>>>(p);
-    else rms_norm_bwd_kernel<T, 8, 2, 256><<<b.blocks, block, smem, s>>>(p);
+  if (vec && b.vpt == 2) {
+    if (b.tpr > 512) rms_norm_bwd_kernel<T, VEC, 2, 1024><<<blocks, block, smem, s>>>(p);
+    else if (b.tpr > 256) rms_norm_bwd_kernel<T, VEC, 2, 512><<<blocks, block, smem, s>>>(p);
+    else rms_norm_bwd_kernel<T, VEC, 2, 256><<<blocks, block, smem, s>>>(p);
+  } else if (vec) {
+    if constexpr (VEC == 4) rms_norm_bwd_kernel<T, VEC, 4, 1024><<<blocks, block, smem, s>>>(p);
   } else if (b.vpt == 4) {
-    if (wide) rms_norm_bwd_kernel<T, 1, 4, 1024><<<b.blocks, block, smem, s>>>(p);
-    else rms_norm_bwd_kernel<T, 1, 4, 256><<<b.blocks, block, smem, s>>>(p);
+    if (b.tpr > 512) rms_norm_bwd_kernel<T, 1, 4, 1024><<<blocks, block, smem, s>>>(p);
+    else if (b.tpr > 256) rms_norm_bwd_kernel<T, 1, 4, 512><<<blocks, block, smem, s>>>(p);
+    else rms_norm_bwd_kernel<T, 1, 4, 256><<<blocks, block, smem, s>>>(p);
   } else {
-    rms_norm_bwd_kernel<T, 1, 16, 1024><<<b.blocks, block, smem, s>>>(p);
+    rms_norm_bwd_kernel<T, 1, 16, 1024><<<blocks, block, smem, s>>>(p);
   }
-  return cudaSuccess;
 }
 
 }  // namespace
@@ -367,8 +486,8 @@ int jla_rms_norm_fwd(int dtype, int64_t rows, int dim, const void* x, const void
   RmsParams p{};
   p.rows = rows, p.dim = dim, p.x = x, p.residual = residual, p.w = weight, p.eps = eps, p.y = y, p.stream = stream_out;
   p.rstd = rstd, p.scale = scale;
-  const bool vec = dim % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(y) &&
-                   aligned16(stream_out);
+  const bool vec = dim % (dtype == JLA_DTYPE_F32 ? 4 : 8) == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) &&
+                   aligned16(y) && aligned16(stream_out);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   {
     ProfScope scope(kProfRmsNorm, s);
@@ -384,8 +503,12 @@ int jla_rms_norm_fwd(int dtype, int64_t rows, int dim, const void* x, const void
 
 size_t jla_rms_norm_bwd_scratch_bytes(int64_t rows, int dim) {
   if (problem(JLA_DTYPE_F32, rows, dim) || rows == 0) return 0;
-  const int a = bwd_shape(rows, dim, false).blocks, b = dim % 8 == 0 ? bwd_shape(rows, dim, true).blocks : 0;
-  return (size_t)(a > b ? a : b) * dim * sizeof(float);
+  int most = bwd_blocks(rows, bwd_shape(dim, 1));
+  for (int vec = 4; vec <= 8; vec += 4) {
+    const int n = dim % vec == 0 ? bwd_blocks(rows, bwd_shape(dim, vec)) : 0;
+    most = n > most ? n : most;
+  }
+  return (size_t)most * dim * sizeof(float);
 }
 
 int jla_rms_norm_bwd(int dtype, int64_t rows, int dim, const void* x, const void* residual, const float* rstd,
@@ -412,19 +535,21 @@ int jla_rms_norm_bwd(int dtype, int64_t rows, int dim, const void* x, const void
   p.rows = rows, p.dim = dim, p.x = x, p.residual = residual, p.rstd = const_cast<float*>(rstd), p.w = weight, p.dy = dy;
   p.dstream = dstream;
   p.dx = dx, p.partial = dweight ? static_cast<float*>(scratch) : nullptr;
-  const bool vec = dim % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(dy) &&
-                   aligned16(dstream) && aligned16(dx) && aligned16(scratch);
-  const BwdShape b = bwd_shape(rows, dim, vec);
+  const int width = dtype == JLA_DTYPE_F32 ? 4 : 8;
+  const bool vec = dim % width == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(dy) &&
+                   aligned16(dstream) && aligned16(dx);
+  const RowShape b = bwd_shape(dim, vec ? width : 1);
+  const int blocks = bwd_blocks(rows, b);
   {
     ProfScope scope(kProfRmsNormBwd, s);
     switch (dtype) {
-      case JLA_DTYPE_BF16: JLA_CUDA_OK(launch_bwd<__nv_bfloat16>(p, b, vec, s)); break;
-      case JLA_DTYPE_F16: JLA_CUDA_OK(launch_bwd<__half>(p, b, vec, s)); break;
-      default: JLA_CUDA_OK(launch_bwd<float>(p, b, vec, s)); break;
+      case JLA_DTYPE_BF16: launch_bwd<__nv_bfloat16>(p, b, blocks, vec, s); break;
+      case JLA_DTYPE_F16: launch_bwd<__half>(p, b, blocks, vec, s); break;
+      default: launch_bwd<float>(p, b, blocks, vec, s); break;
     }
   }
   JLA_LAUNCH_OK();
-  return dweight ? column_sums(p.partial, b.blocks, dim, dweight, s) : JLA_OK;
+  return dweight ? column_sums(p.partial, blocks, dim, dweight, s) : JLA_OK;
 }
 
 }  // extern "C"
