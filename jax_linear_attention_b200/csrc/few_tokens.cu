@@ -1,5 +1,5 @@
-// Matrix products of few tokens (a decoding step, a short prompt) with the epilogue fused: the same results as
-// product_tc.cu, for calls whose time is that of reading the weights.
+// Matrix products of few tokens (a decoding step, a short prompt) or few features with the epilogue fused: what
+// product_tc.cu computes, for calls whose time is that of reading the weights.
 //
 // Bound by HBM, so the weights have to stream through as many SMs as there are. The roles of the operands are swapped: 128
 // features (rows of W) fill the 128 TMEM lanes, BN tokens are the accumulator's columns, so that few tokens waste
@@ -374,9 +374,7 @@ int launch(const Product& p, int device, int sms, cudaStream_t s) {
 }
 
 template <bool W_MN, bool FP8, bool GATED>
-int pick(const Product& p, cudaStream_t s) {
-  int dev = 0, sms = 0;
-  if (const int rc = current_device(&dev, &sms)) return rc;
+int pick(const Product& p, int dev, int sms, cudaStream_t s) {
   if (p.rows <= 16) return launch<16, W_MN, FP8, GATED>(p, dev, sms, s);
   if (p.rows <= 32) return launch<32, W_MN, FP8, GATED>(p, dev, sms, s);
   if (p.rows <= 64) return launch<64, W_MN, FP8, GATED>(p, dev, sms, s);
@@ -386,12 +384,28 @@ int pick(const Product& p, cudaStream_t s) {
 
 }  // namespace
 
-bool few_tokens_applies(const Product& p) { return !p.x_mn && !p.group && p.rows <= 256; }
+// Up to 64 tokens always; up to 2048 where this kernel is expected to be the faster one. Measured, in us, inputs from HBM:
+//   this kernel: 8.0 + 0.34 a step of its longest CTA (gated 8.6 + 0.48)     pairs: 6.2 + 0.21 a step of the busiest pair
+//   4096 -> 256, 512 tokens: 10.7 against 18.7     4096 -> 2048, 256: 14.5, 20.2     1024 -> 1024, 256: 8.8, 9.7
+//   512 -> 4096, 128: 9.1, 8.7     2048 -> 6144, 256: 18.6, 14.8     gated 2048 -> 6144, 256: 40.9, 21.3
+bool few_tokens_applies(const Product& p, int sms) {
+  if (p.x_mn || p.group || p.rows > 2048) return false;
+  if (p.rows <= 64) return true;
+  const int kb = p.dtype == JLA_DTYPE_E4M3 ? 128 : 64, kt = (p.depth + kb - 1) / kb * (p.pair ? 2 : 1);
+  const int bn = p.gated ? 64 : 128, tiles = (p.features + 127) / 128 * (int)((p.rows + bn - 1) / bn);
+  int split = sms / tiles < kMaxSplit ? sms / tiles : kMaxSplit;
+  split = split > kt / 2 ? kt / 2 : split;
+  split = split < 1 ? 1 : split;
+  const int steps = (kt + split - 1) / split * ((tiles * split + sms - 1) / sms);
+  const int cols = p.features * (p.gated ? 2 : 1);
+  const int pair_steps = ((int)((p.rows + 255) / 256) * ((cols + 255) / 256) + sms / 2 - 1) / (sms / 2) * kt;
+  return (p.gated ? 860 + 48 * steps : 800 + 34 * steps) < 620 + 21 * pair_steps;
+}
 
-int product_few_tokens(const Product& p, cudaStream_t s) {
-  if (p.dtype == JLA_DTYPE_E4M3) return p.gated ? pick<false, true, true>(p, s) : pick<false, true, false>(p, s);
-  if (p.w_mn) return pick<true, false, false>(p, s);
-  return p.gated ? pick<false, false, true>(p, s) : pick<false, false, false>(p, s);
+int product_few_tokens(const Product& p, int dev, int sms, cudaStream_t s) {
+  if (p.dtype == JLA_DTYPE_E4M3) return p.gated ? pick<false, true, true>(p, dev, sms, s) : pick<false, true, false>(p, dev, sms, s);
+  if (p.w_mn) return pick<true, false, false>(p, dev, sms, s);
+  return p.gated ? pick<false, false, true>(p, dev, sms, s) : pick<false, false, false>(p, dev, sms, s);
 }
 
 }  // namespace jla

@@ -86,9 +86,9 @@ struct Product {
   float* save[2] = {};   // z, or g and u, in float32 for a later backward pass
 };
 
-int product_pairs(const Product& p, cudaStream_t stream);       // product_tc.cu: any number of tokens
-int product_few_tokens(const Product& p, cudaStream_t stream);  // few_tokens.cu: at most kFewTokens
-bool few_tokens_applies(const Product& p);
+int product_pairs(const Product& p, int device, int sms, cudaStream_t stream);       // product_tc.cu: any number of tokens
+int product_few_tokens(const Product& p, int device, int sms, cudaStream_t stream);  // few_tokens.cu: where few_tokens_applies
+bool few_tokens_applies(const Product& p, int sms);
 
 int* tc_status_ptr();  // status.cu
 

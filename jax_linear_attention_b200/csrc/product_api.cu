@@ -60,7 +60,9 @@ int run(const Product& p, cudaStream_t s) {
                         static_cast<const void*>(p.save[1])}) {
     if (!aligned16(q)) return refuse("linear: pointers must be 16-byte aligned");
   }
-  return few_tokens_applies(p) ? product_few_tokens(p, s) : product_pairs(p, s);
+  int device = 0, sms = 0;
+  if (const int rc = current_device(&device, &sms)) return rc;
+  return few_tokens_applies(p, sms) ? product_few_tokens(p, device, sms, s) : product_pairs(p, device, sms, s);
 }
 
 }  // namespace

@@ -4,6 +4,6 @@ norm; and what stands around a mixer in a block: the residual stream's RMS norm,
 feed-forward block."""
 from .conv import short_conv  # noqa: F401
 from .gates import gate_prologue  # noqa: F401
-from .linear import gated_linear, linear  # noqa: F401
 from .norm import gated_rms_norm, rms_norm  # noqa: F401
+from .products import gated_linear, linear  # noqa: F401
 from .ssm import mamba2_ssd  # noqa: F401

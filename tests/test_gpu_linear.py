@@ -130,15 +130,23 @@ def test_linear_gradients(rows, depth, out, dtype, act, bias, residual):
     _check_linear_gradients(rows, depth, out, DTYPES[dtype], act, bias, residual)
 
 
-# Sizes at which the pairs of CTAs take tiles of 256 columns (above they take 128): 74 tiles of 256 x 256, one for each pair.
-def test_wide_tiles_forward():
-    t = _inputs(18900, 72, 256, torch.bfloat16, bias=True, residual=True)
+# Every kernel and tile width: few tokens (16, 32, 64 or 128 of them a block), pairs of CTAs (128 or 256 columns a tile, one
+# tile a pair and several).
+KERNELS = [(5, 2048, 136), (20, 520, 200), (50, 1000, 72), (100, 2048, 264), (100, 72, 2000), (1500, 4096, 24), (2100, 72, 56),
+           (2100, 264, 72), (2100, 136, 136), (5000, 72, 1000), (18900, 72, 256)]
+
+
+@pytest.mark.parametrize("rows, depth, out", KERNELS)
+def test_every_kernel(rows, depth, out):
+    t = _inputs(rows, depth, out, torch.bfloat16, bias=True, residual=True)
     _check_linear(t, "silu", layers.linear(t["x"], t["w"], t["b"], activation="silu", residual=t["r"]), torch.bfloat16)
+    _check_linear_gradients(rows, depth, out, torch.bfloat16, "silu", True, True)
+    _check_linear_gradients(rows, depth, out, torch.float16, None, False, False)
 
 
-def test_wide_tiles_gradients():
-    _check_linear_gradients(100, 1792, 2560, torch.float16, None, False, False)   # dW: 10 x 7 tiles
-    _check_linear_gradients(18900, 256, 72, torch.bfloat16, "silu", False, False)  # dx: 74 x 1 tiles
+def test_weight_gradients_of_many_tiles():
+    _check_linear_gradients(100, 1792, 2560, torch.float16, None, False, False)  # 70 tiles
+    _check_linear_gradients(100, 2048, 4096, torch.bfloat16, None, False, False)  # 128
 
 
 def _gated64(x, w, up, act):
@@ -190,8 +198,12 @@ def test_gated_gradients(rows, depth, out, act, dtype):
     _check_gated(rows, depth, out, DTYPES[dtype], act, True)
 
 
-def test_gated_wide_tiles():
-    _check_gated(18900, 72, 128, torch.bfloat16, "silu", True)
+@pytest.mark.parametrize("rows, depth, out", KERNELS)
+def test_gated_every_kernel(rows, depth, out):
+    _check_gated(rows, depth, out, torch.bfloat16, "silu", True)
+
+
+def test_gated_weight_gradients_of_many_tiles():
     _check_gated(70, 1792, 1280, torch.float16, "silu", True)  # dWg and dWu: 2 x 5 x 7 tiles
 
 
@@ -201,7 +213,8 @@ def _e4m3(x):
 
 
 @pytest.mark.parametrize("rows, depth, out", [(1, 64, 64), (1, 16, 8), (5, 2048, 136), (33, 208, 1000), (100, 4096, 72),
-                                              (200, 144, 264), (300, 16, 200), (1003, 1024, 520), (18900, 80, 256)])
+                                              (200, 144, 264), (300, 16, 200), (1003, 1024, 520), (18900, 80, 256),
+                                              (20, 4096, 136), (60, 4096, 136), (2100, 80, 56), (5000, 144, 1000)])
 @pytest.mark.parametrize("out_dtype", DTYPES)
 def test_e4m3(rows, depth, out, out_dtype):
     dtype = DTYPES[out_dtype]
