@@ -55,6 +55,7 @@ class BwdIO(C.Structure):
 
 
 _lib = None
+_torch_ops = None
 
 
 def load() -> C.CDLL:
@@ -118,6 +119,26 @@ def load() -> C.CDLL:
     lib.jla_selftest_bounded_wait.argtypes = [C.c_uint32, C.c_void_p]
     _lib = lib
     return lib
+
+
+def torch_ops():
+    """The extension module of ``csrc/torch_ops.cpp``, bound to the entry points of the loaded library; raises if it has not
+    been built."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib = load()
+        try:
+            from . import _torch_ops as module
+        except ImportError as err:
+            raise RuntimeError(
+                "the torch side of the layers (_torch_ops.so) is missing or was built for another torch: build it with "
+                f"`python -m jax_linear_attention_b200.build` (there is no other path): {err}") from err
+        module.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in (
+            "jla_last_error", "jla_rms_norm_fwd", "jla_rms_norm_bwd_scratch_bytes", "jla_rms_norm_bwd", "jla_linear_fwd",
+            "jla_gated_linear_fwd", "jla_activation_bwd_scratch_bytes", "jla_activation_bwd", "jla_gated_activation_bwd",
+            "jla_linear_bwd_input", "jla_linear_bwd_weight")})
+        _torch_ops = module
+    return _torch_ops
 
 
 def launch(name: str, device, *args) -> None:

@@ -3,7 +3,8 @@
     python -m jax_linear_attention_b200.build [--force] [--verbose]
 
 Every ``csrc/*.cu`` is compiled to an object (in parallel, only when its sources are newer than the
-object) and linked into ``jax_linear_attention_b200/libjla_b200.so``. No GPU is needed to build.
+object) and linked into ``jax_linear_attention_b200/libjla_b200.so``; ``csrc/torch_ops.cpp`` (the torch side of the layers
+whose host time matters most) becomes ``_torch_ops.so`` next to it. No GPU is needed to build.
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libjla_b200.so")
+TORCH_OPS = os.path.join(HERE, "_torch_ops.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -54,6 +56,27 @@ def _compile(src: str, obj: str, verbose: bool) -> str:
     return obj
 
 
+def _build_torch_ops(verbose: bool) -> str:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], cuda]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_ops",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f for path in includes for f in ("-isystem", path)), os.path.join(CSRC, "torch_ops.cpp"), "-o", TORCH_OPS,
+           *(f"-L{path}" for path in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+           "-ltorch_python"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"the torch side of the layers failed to build:\n{(proc.stdout + proc.stderr)[-6000:]}")
+    if verbose:
+        print(proc.stdout + proc.stderr)
+    return TORCH_OPS
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     sources = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
@@ -68,9 +91,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
     stale = set(glob.glob(os.path.join(OBJ, "*.o"))) - set(objs)
     for path in stale:
         os.remove(path)
-    if jobs:
-        with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(jobs))) as pool:
-            list(pool.map(lambda j: _compile(j[0], j[1], verbose), jobs))
+    with concurrent.futures.ThreadPoolExecutor(max_workers=8) as pool:
+        side = [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(HERE, "..", "include", "jla_b200.h")]
+        glue = pool.submit(_build_torch_ops, verbose) if force or _newer(TORCH_OPS, side) else None
+        list(pool.map(lambda j: _compile(j[0], j[1], verbose), jobs))
+        if glue is not None:
+            glue.result()
     if jobs or stale or force or _newer(LIB, objs):
         cmd = [nvcc(), "-shared", "-o", LIB, *objs, "-lcudart"]
         proc = subprocess.run(cmd, capture_output=True, text=True)

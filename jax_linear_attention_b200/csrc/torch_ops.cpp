@@ -1,0 +1,472 @@
+// The torch side of rms_norm, linear and gated_linear: what a call of layers.* does on the host besides the launch, in C++.
+//
+// A decoding step calls these operators a few times a layer with kernels of a few microseconds, and a small training step's
+// gradients come back through autograd's device thread: there the host bounds the call. Argument checks, output
+// allocation and autograd nodes in Python cost 14 us a call forward and 75 us for a gradient; here they cost 5 and 45 (of
+// which 40 are autograd's own hand-over between threads).
+//
+// The kernels are reached through the C ABI (include/jla_b200.h) of the library that the Python side has loaded: bind() gets
+// the addresses of its entry points. A call that these functions do not take comes back as None, and the Python side
+// says what is wrong with it.
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <string>
+
+#include "../../include/jla_b200.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+constexpr at::ScalarType kNone = at::ScalarType::Undefined;  // "no dtype asked for"
+
+struct Abi {
+  decltype(&jla_last_error) last_error;
+  decltype(&jla_rms_norm_fwd) rms_norm_fwd;
+  decltype(&jla_rms_norm_bwd_scratch_bytes) rms_norm_bwd_scratch_bytes;
+  decltype(&jla_rms_norm_bwd) rms_norm_bwd;
+  decltype(&jla_linear_fwd) linear_fwd;
+  decltype(&jla_gated_linear_fwd) gated_linear_fwd;
+  decltype(&jla_activation_bwd_scratch_bytes) activation_bwd_scratch_bytes;
+  decltype(&jla_activation_bwd) activation_bwd;
+  decltype(&jla_gated_activation_bwd) gated_activation_bwd;
+  decltype(&jla_linear_bwd_input) linear_bwd_input;
+  decltype(&jla_linear_bwd_weight) linear_bwd_weight;
+} abi;
+
+void bind(const py::dict& addresses) {
+  auto at = [&](const char* name) { return reinterpret_cast<void*>(addresses[name].cast<uintptr_t>()); };
+#define JLA_BIND(name) abi.name = reinterpret_cast<decltype(abi.name)>(at("jla_" #name))
+  JLA_BIND(last_error);
+  JLA_BIND(rms_norm_fwd);
+  JLA_BIND(rms_norm_bwd_scratch_bytes);
+  JLA_BIND(rms_norm_bwd);
+  JLA_BIND(linear_fwd);
+  JLA_BIND(gated_linear_fwd);
+  JLA_BIND(activation_bwd_scratch_bytes);
+  JLA_BIND(activation_bwd);
+  JLA_BIND(gated_activation_bwd);
+  JLA_BIND(linear_bwd_input);
+  JLA_BIND(linear_bwd_weight);
+#undef JLA_BIND
+}
+
+void check(int rc, const char* what) {
+  if (rc == JLA_OK) return;
+  const std::string text = std::string(what) + ": " + abi.last_error();
+  TORCH_CHECK_NOT_IMPLEMENTED(rc != JLA_ERR_UNSUPPORTED, text);
+  TORCH_CHECK_VALUE(rc != JLA_ERR_BAD_ARGUMENT && rc != JLA_ERR_WORKSPACE, text);
+  TORCH_CHECK(false, text, " (status ", rc, ")");
+}
+
+int code(at::ScalarType t) {
+  switch (t) {
+    case at::kBFloat16: return JLA_DTYPE_BF16;
+    case at::kHalf: return JLA_DTYPE_F16;
+    case at::kFloat: return JLA_DTYPE_F32;
+    case at::kFloat8_e4m3fn: return JLA_DTYPE_E4M3;
+    default: return -1;
+  }
+}
+bool sixteen(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+const float* fptr(const Tensor& t) { return static_cast<const float*>(ptr(t)); }
+float* fmut(const Tensor& t) { return static_cast<float*>(ptr(t)); }
+jla_stream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+// Contiguous and on a 16-byte boundary (a slice of another tensor may start anywhere).
+Tensor aligned(const Tensor& t) {
+  if (!t.defined()) return t;
+  Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) & 15 ? c.clone() : c;
+}
+
+// x [..., width] as rows that start `stride` elements apart, without a copy where they allow 16-byte loads.
+struct Rows {
+  Tensor t;
+  int64_t rows, stride;
+};
+Rows rows_of(const Tensor& x, int64_t width) {
+  const int64_t rows = x.numel() / width, last = x.dim() - 1;
+  if (!x.is_contiguous() && x.stride(last) == 1) {
+    int64_t stride = -1, next = 0;
+    bool even = true;
+    for (int64_t i = last - 1; i >= 0 && even; --i) {
+      if (x.size(i) == 1) continue;
+      if (stride < 0) stride = x.stride(i), next = stride * x.size(i);
+      else if (x.stride(i) == next) next *= x.size(i);
+      else even = false;
+    }
+    if (stride < 0) stride = width;
+    if (even && stride >= width && !((stride * x.element_size() | reinterpret_cast<intptr_t>(x.data_ptr())) & 15)) {
+      return {x, rows, stride};
+    }
+  }
+  return {aligned(x), rows, width};
+}
+
+// Whether a gradient would be recorded, of any order or mode, for a call with these tensors.
+bool differentiated(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors) {
+    if (!t->defined()) continue;
+    if (t->requires_grad() && at::GradMode::is_enabled()) return true;
+    if (t->_fw_grad(0).defined()) return true;
+  }
+  return false;
+}
+
+// Gradients that cannot be differentiated again: an attempt raises, as torch's once_differentiable does.
+variable_list once(variable_list grads) {
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    auto error = std::make_shared<torch::autograd::DelayedError>("the gradients of this operator cannot be differentiated again", 1);
+    g = (*error)(variable_list{g})[0];
+  }
+  return grads;
+}
+
+// A tensor, None (undefined) or something else (false).
+bool take(const py::handle& h, Tensor& t) {
+  if (h.is_none()) return true;
+  if (!THPVariable_Check(h.ptr())) return false;
+  t = THPVariable_Unpack(h.ptr());
+  return true;
+}
+// None or a torch.dtype.
+bool take_dtype(const py::handle& h, at::ScalarType& t) {
+  if (h.is_none()) return true;
+  if (!THPDtype_Check(h.ptr())) return false;
+  t = reinterpret_cast<THPDtype*>(h.ptr())->scalar_type;
+  return true;
+}
+bool on(const Tensor& t, const Tensor& like) { return t.is_cuda() && t.get_device() == like.get_device(); }
+
+// (a node's inputs that are not there are left out of its edges: needs_input_grad counts the others only)
+std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+  return at::empty(shape, like.options().dtype(type).requires_grad(false));
+}
+
+// ---- rms_norm -----------------------------------------------------------------------------------------------------------
+
+struct Norm {
+  Tensor y, stream, rstd, scale;
+};
+
+Norm norm_fwd(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, bool e4m3, bool keep) {
+  c10::cuda::OptionalCUDAGuard guard(x.device());
+  Norm n;
+  const int64_t dim = x.size(-1), rows = x.numel() / dim;
+  n.y = make(x.sizes(), e4m3 ? at::kFloat8_e4m3fn : x.scalar_type(), x);
+  if (residual.defined()) n.stream = make(x.sizes(), x.scalar_type(), x);
+  if (keep) n.rstd = make({rows}, at::kFloat, x);
+  if (e4m3) n.scale = make(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+  check(abi.rms_norm_fwd(code(x.scalar_type()), rows, (int)dim, ptr(x), ptr(residual), fptr(weight), (float)eps, e4m3, ptr(n.y),
+                         ptr(n.stream), fmut(n.rstd), fmut(n.scale), stream_of(x)),
+        "jla_rms_norm_fwd");
+  return n;
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& residual_,
+                               double eps) {
+    const Tensor residual = residual_.value_or(Tensor());
+    Norm n = norm_fwd(x, residual, weight, eps, false, true);
+    ctx->save_for_backward({x, residual, weight, n.rstd});
+    ctx->set_materialize_grads(false);
+    if (!residual.defined()) return {n.y};
+    if (!x.requires_grad() && !residual.requires_grad()) ctx->mark_non_differentiable({n.stream});  // the weight is not in it
+    return {n.y, n.stream};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool again = at::GradMode::is_enabled();
+    variable_list out;
+    {
+      at::AutoGradMode off(false);
+      const variable_list saved = ctx->get_saved_variables();
+      const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2], &rstd = saved[3];
+      Tensor dx, dw, dy = grads[0], ds = grads.size() > 1 ? grads[1] : Tensor();
+      if (!dy.defined()) {
+        dx = ds;  // only the stream was used
+      } else {
+        c10::cuda::OptionalCUDAGuard guard(x.device());
+        dy = aligned(dy), ds = aligned(ds);
+        const int64_t dim = x.size(-1), rows = x.numel() / dim;
+        dx = make(x.sizes(), x.scalar_type(), x);
+        Tensor scratch;
+        size_t bytes = 0;
+        if (ctx->needs_input_grad(1)) {
+          dw = make({dim}, at::kFloat, x);
+          bytes = abi.rms_norm_bwd_scratch_bytes(rows, (int)dim);
+          scratch = make({(int64_t)bytes}, at::kByte, x);
+        }
+        check(abi.rms_norm_bwd(code(x.scalar_type()), rows, (int)dim, ptr(x), ptr(residual), fptr(rstd), fptr(weight), ptr(dy),
+                               ptr(ds), ptr(dx), fmut(dw), ptr(scratch), bytes, stream_of(x)),
+              "jla_rms_norm_bwd");
+      }
+      out = {dx, dw, residual.defined() ? dx : Tensor(), Tensor()};
+    }
+    return again ? once(out) : out;
+  }
+};
+
+// y, (y, stream), (q, scale) or (q, scale, stream); None for a call that the Python side has to refuse.
+py::object rms_norm(const py::handle& x_, const py::handle& weight_, const py::handle& residual_, double eps,
+                    const py::handle& dtype_) {
+  Tensor x, weight, residual;
+  at::ScalarType out = kNone;
+  if (!take(x_, x) || !take(weight_, weight) || !take(residual_, residual) || !take_dtype(dtype_, out)) return py::none();
+  if (!x.defined() || !weight.defined() || !x.is_cuda() || x.dim() < 1) return py::none();
+  const int64_t dim = x.size(-1);
+  const at::ScalarType type = x.scalar_type();
+  if (dim < 1 || dim > 16384 || code(type) < 0 || code(type) == JLA_DTYPE_E4M3 || weight.dim() != 1 || weight.size(0) != dim ||
+      !on(weight, x) || !weight.is_floating_point()) {
+    return py::none();
+  }
+  if (residual.defined() && (residual.scalar_type() != type || !on(residual, x) || residual.sizes() != x.sizes())) return py::none();
+  const bool e4m3 = out == at::kFloat8_e4m3fn, grads = differentiated({&x, &weight, &residual});
+  if ((out != kNone && !e4m3 && out != type) || (e4m3 && grads)) return py::none();
+  variable_list made;
+  {
+    py::gil_scoped_release unlocked;
+    x = aligned(x), residual = aligned(residual);
+    weight = aligned(weight.scalar_type() == at::kFloat ? weight : weight.to(at::kFloat));
+    if (grads) {
+      made = RmsNorm::apply(x, weight, maybe(residual), eps);
+    } else {
+      Norm n = norm_fwd(x, residual, weight, eps, e4m3, false);
+      made.push_back(n.y);
+      if (e4m3) made.push_back(n.scale);
+      if (n.stream.defined()) made.push_back(n.stream);
+    }
+  }
+  if (made.size() == 1) return py::cast(made[0]);
+  if (made.size() == 2) return py::make_tuple(made[0], made[1]);
+  return py::make_tuple(made[0], made[1], made[2]);
+}
+
+// ---- linear and gated_linear ------------------------------------------------------------------------------------------------
+
+std::vector<int64_t> out_shape(const Tensor& x, int64_t out) {
+  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+  s.back() = out;
+  return s;
+}
+
+Tensor linear_fwd(const Rows& x, const Tensor& weight, const Tensor& x_scale, const Tensor& w_scale, const Tensor& bias, int64_t act,
+                  const Tensor& residual, at::IntArrayRef shape, at::ScalarType type, Tensor* z) {
+  c10::cuda::OptionalCUDAGuard guard(weight.device());
+  Tensor y = make(shape, type, weight);
+  if (z) *z = make({x.rows, weight.size(0)}, at::kFloat, weight);
+  check(abi.linear_fwd(code(weight.scalar_type()), code(type), x.rows, (int)weight.size(1), (int)weight.size(0), ptr(x.t), x.stride,
+                       ptr(weight), fptr(x_scale), fptr(w_scale), fptr(bias), (int)act, ptr(residual), ptr(y), z ? fmut(*z) : nullptr,
+                       stream_of(weight)),
+        "jla_linear_fwd");
+  return y;
+}
+
+Tensor gated_fwd(const Rows& x, const Tensor& gate, const Tensor& up, const Tensor& x_scale, const Tensor& g_scale,
+                 const Tensor& u_scale, int64_t act, at::IntArrayRef shape, at::ScalarType type, Tensor* g, Tensor* u) {
+  c10::cuda::OptionalCUDAGuard guard(gate.device());
+  Tensor h = make(shape, type, gate);
+  if (g) *g = make({x.rows, gate.size(0)}, at::kFloat, gate), *u = make({x.rows, gate.size(0)}, at::kFloat, gate);
+  check(abi.gated_linear_fwd(code(gate.scalar_type()), code(type), x.rows, (int)gate.size(1), (int)gate.size(0), ptr(x.t), x.stride,
+                             ptr(gate), ptr(up), fptr(x_scale), fptr(g_scale), fptr(u_scale), (int)act, ptr(h),
+                             g ? fmut(*g) : nullptr, g ? fmut(*u) : nullptr, stream_of(gate)),
+        "jla_gated_linear_fwd");
+  return h;
+}
+
+Tensor input_grad(at::IntArrayRef shape, int64_t rows, const Tensor& dz, const Tensor& w, const Tensor& dz2, const Tensor& w2) {
+  Tensor dx = make(shape, w.scalar_type(), w);
+  check(abi.linear_bwd_input(code(w.scalar_type()), rows, (int)w.size(1), (int)w.size(0), ptr(dz), ptr(w), ptr(dz2), ptr(w2), ptr(dx),
+                             stream_of(w)),
+        "jla_linear_bwd_input");
+  return dx;
+}
+
+// dw of dz, and dw2 of dz2 in the same launch where there is one
+void weight_grads(const Tensor& w, int64_t rows, const Tensor& x, int64_t stride, const Tensor& dz, Tensor& dw, const Tensor& dz2,
+                  Tensor* dw2) {
+  dw = make(w.sizes(), w.scalar_type(), w);
+  if (dw2) *dw2 = make(w.sizes(), w.scalar_type(), w);
+  check(abi.linear_bwd_weight(code(w.scalar_type()), rows, (int)w.size(1), (int)w.size(0), ptr(dz), ptr(dz2), ptr(x), stride, ptr(dw),
+                              dw2 ? ptr(*dw2) : nullptr, stream_of(w)),
+        "jla_linear_bwd_weight");
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_,
+                        const std::optional<Tensor>& residual_, int64_t act) {
+    const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
+    const Rows rows = rows_of(x, weight.size(1));
+    Tensor z;
+    Tensor y = linear_fwd(rows, weight, {}, {}, bias, act, aligned(residual), out_shape(x, weight.size(0)), x.scalar_type(),
+                          act != JLA_ACT_NONE ? &z : nullptr);
+    ctx->save_for_backward({rows.t, weight, z});
+    ctx->saved_data["cfg"] = std::vector<int64_t>{act, rows.rows, rows.stride, bias.defined(), residual.defined()};
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool again = at::GradMode::is_enabled();
+    variable_list out;
+    {
+      at::AutoGradMode off(false);
+      const variable_list saved = ctx->get_saved_variables();
+      const Tensor &x = saved[0], &weight = saved[1], &z = saved[2];
+      const std::vector<int64_t> cfg = ctx->saved_data["cfg"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
+      const int64_t act = cfg[0], rows = cfg[1];
+      const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = cfg[3] && ctx->needs_input_grad(2);
+      c10::cuda::OptionalCUDAGuard guard(weight.device());
+      const Tensor dy = aligned(grads[0]);
+      Tensor dz = dy, db, dx, dw;
+      if (need_b || (z.defined() && (need_x || need_w))) {
+        const int64_t n = weight.size(0);
+        if (z.defined()) dz = make({rows, n}, weight.scalar_type(), weight);
+        Tensor scratch;
+        size_t bytes = 0;
+        if (need_b) {
+          bytes = abi.activation_bwd_scratch_bytes(rows, (int)n);
+          db = make({n}, at::kFloat, weight);
+          scratch = make({(int64_t)bytes}, at::kByte, weight);
+        }
+        check(abi.activation_bwd(code(weight.scalar_type()), rows, (int)n, (int)act, fptr(z), ptr(dy), z.defined() ? ptr(dz) : nullptr,
+                                 fmut(db), ptr(scratch), bytes, stream_of(weight)),
+              "jla_activation_bwd");
+      }
+      if (need_x) dx = input_grad(shape, rows, dz, weight, {}, {});
+      if (need_w) weight_grads(weight, rows, x, cfg[2], dz, dw, {}, nullptr);
+      out = {dx, dw, db, cfg[4] && ctx->needs_input_grad(cfg[3] ? 3 : 2) ? grads[0] : Tensor(), Tensor()};
+    }
+    return again ? once(out) : out;
+  }
+};
+
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& up, int64_t act) {
+    const Rows rows = rows_of(x, gate.size(1));
+    Tensor g, u;
+    Tensor h = gated_fwd(rows, gate, up, {}, {}, {}, act, out_shape(x, gate.size(0)), x.scalar_type(), &g, &u);
+    ctx->save_for_backward({rows.t, gate, up, g, u});
+    ctx->saved_data["cfg"] = std::vector<int64_t>{act, rows.rows, rows.stride};
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return h;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool again = at::GradMode::is_enabled();
+    variable_list out;
+    {
+      at::AutoGradMode off(false);
+      const variable_list saved = ctx->get_saved_variables();
+      const Tensor &x = saved[0], &gate = saved[1], &up = saved[2], &g = saved[3], &u = saved[4];
+      const std::vector<int64_t> cfg = ctx->saved_data["cfg"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
+      const int64_t rows = cfg[1], n = gate.size(0);
+      c10::cuda::OptionalCUDAGuard guard(gate.device());
+      const Tensor dh = aligned(grads[0]);
+      const Tensor dg = make({rows, n}, gate.scalar_type(), gate), du = make({rows, n}, gate.scalar_type(), gate);
+      check(abi.gated_activation_bwd(code(gate.scalar_type()), rows, (int)n, (int)cfg[0], fptr(g), fptr(u), ptr(dh), ptr(dg), ptr(du),
+                                     stream_of(gate)),
+            "jla_gated_activation_bwd");
+      Tensor dx, d_gate, d_up;
+      const bool need_g = ctx->needs_input_grad(1), need_u = ctx->needs_input_grad(2);
+      if (ctx->needs_input_grad(0)) dx = input_grad(shape, rows, dg, gate, du, up);
+      if (need_g) weight_grads(gate, rows, x, cfg[2], dg, d_gate, need_u ? du : Tensor(), need_u ? &d_up : nullptr);
+      else if (need_u) weight_grads(up, rows, x, cfg[2], du, d_up, {}, nullptr);
+      out = {dx, d_gate, d_up, Tensor()};
+    }
+    return again ? once(out) : out;
+  }
+};
+
+// The checks that both products share; `type` becomes the output's dtype.
+bool operands(const Tensor& x, const Tensor& w, const Tensor& x_scale, std::initializer_list<const Tensor*> scales,
+              const py::handle& dtype_, at::ScalarType& type) {
+  if (!x.defined() || !w.defined() || !x.is_cuda() || !on(w, x) || x.dim() < 1 || w.dim() != 2) return false;
+  const at::ScalarType t = x.scalar_type();
+  const int64_t out = w.size(0), depth = w.size(1), step = t == at::kFloat8_e4m3fn ? 16 : 8;
+  if (w.scalar_type() != t || x.size(-1) != depth || depth < step || depth % step || out < 8 || out % 8) return false;
+  type = kNone;
+  if (!take_dtype(dtype_, type)) return false;
+  if (t != at::kFloat8_e4m3fn) {
+    for (const Tensor* s : scales) {
+      if (s->defined()) return false;
+    }
+    if (!sixteen(t) || x_scale.defined() || (type != kNone && type != t)) return false;
+    type = t;
+    return true;
+  }
+  for (const Tensor* s : scales) {
+    if (!s->defined() || s->scalar_type() != at::kFloat || s->dim() != 1 || s->size(0) != out || !on(*s, x)) return false;
+  }
+  if (!x_scale.defined() || x_scale.scalar_type() != at::kFloat || x_scale.sizes() != x.sizes().slice(0, x.dim() - 1) || !on(x_scale, x)) {
+    return false;
+  }
+  if (type == kNone) type = at::kBFloat16;
+  return sixteen(type);
+}
+
+py::object linear(const py::handle& x_, const py::handle& weight_, const py::handle& bias_, int64_t act, const py::handle& residual_,
+                  const py::handle& x_scale_, const py::handle& w_scale_, const py::handle& dtype_) {
+  Tensor x, w, bias, residual, x_scale, w_scale;
+  at::ScalarType type;
+  if (!take(x_, x) || !take(weight_, w) || !take(bias_, bias) || !take(residual_, residual) || !take(x_scale_, x_scale) ||
+      !take(w_scale_, w_scale) || !operands(x, w, x_scale, {&w_scale}, dtype_, type)) {
+    return py::none();
+  }
+  if (bias.defined() && (bias.dim() != 1 || bias.size(0) != w.size(0) || !on(bias, x) || !bias.is_floating_point())) return py::none();
+  const std::vector<int64_t> shape = out_shape(x, w.size(0));
+  if (residual.defined() && (residual.scalar_type() != type || !on(residual, x) || residual.sizes() != at::IntArrayRef(shape))) {
+    return py::none();
+  }
+  const bool grads = differentiated({&x, &w, &bias, &residual, &x_scale, &w_scale});
+  if (grads && x.scalar_type() == at::kFloat8_e4m3fn) return py::none();
+  Tensor y;
+  {
+    py::gil_scoped_release unlocked;
+    w = aligned(w);
+    if (bias.defined()) bias = aligned(bias.scalar_type() == at::kFloat ? bias : bias.to(at::kFloat));
+    y = grads ? Linear::apply(x, w, maybe(bias), maybe(residual), act)
+              : linear_fwd(rows_of(x, w.size(1)), w, aligned(x_scale), aligned(w_scale), bias, act, aligned(residual), shape, type, nullptr);
+  }
+  return py::cast(y);
+}
+
+py::object gated_linear(const py::handle& x_, const py::handle& gate_, const py::handle& up_, int64_t act, const py::handle& x_scale_,
+                        const py::handle& g_scale_, const py::handle& u_scale_, const py::handle& dtype_) {
+  Tensor x, gate, up, x_scale, g_scale, u_scale;
+  at::ScalarType type;
+  if (!take(x_, x) || !take(gate_, gate) || !take(up_, up) || !take(x_scale_, x_scale) || !take(g_scale_, g_scale) ||
+      !take(u_scale_, u_scale) || !operands(x, gate, x_scale, {&g_scale, &u_scale}, dtype_, type) || !up.defined() || !on(up, x) ||
+      up.scalar_type() != gate.scalar_type() || up.sizes() != gate.sizes()) {
+    return py::none();
+  }
+  const bool grads = differentiated({&x, &gate, &up, &x_scale, &g_scale, &u_scale});
+  if (grads && x.scalar_type() == at::kFloat8_e4m3fn) return py::none();
+  Tensor h;
+  {
+    py::gil_scoped_release unlocked;
+    gate = aligned(gate), up = aligned(up);
+    h = grads ? GatedLinear::apply(x, gate, up, act)
+              : gated_fwd(rows_of(x, gate.size(1)), gate, up, aligned(x_scale), aligned(g_scale), aligned(u_scale), act,
+                          out_shape(x, gate.size(0)), type, nullptr, nullptr);
+  }
+  return py::cast(h);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("bind", &bind);
+  m.def("rms_norm", &rms_norm);
+  m.def("linear", &linear);
+  m.def("gated_linear", &gated_linear);
+}

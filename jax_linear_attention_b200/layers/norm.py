@@ -21,7 +21,6 @@ import ctypes as C
 import torch
 
 from .. import _lib
-from ..ops.cuda import aligned, nothing_to_differentiate
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -81,54 +80,6 @@ def gated_rms_norm(x, z, weight, *, eps: float = 1e-6, activation: str = "silu",
                                activation == "sigmoid", bool(norm_before_gate), int(group))
 
 
-class _RMSNorm(torch.autograd.Function):
-    """``(y, stream)``; ``stream`` is None without a residual."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, eps):
-        y, stream, rstd, _ = _rms_norm_fwd(x, residual, weight, eps, False, True)
-        ctx.save_for_backward(x, residual, rstd, weight)
-        ctx.set_materialize_grads(False)
-        if stream is not None and not (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
-            ctx.mark_non_differentiable(stream)  # the weight is not in it
-        return y, stream
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dstream):
-        x, residual, rstd, weight = ctx.saved_tensors
-        if dy is None:  # only the stream was used
-            return dstream, dstream, None, None
-        dim = x.shape[-1]
-        rows = x.numel() // dim
-        dy, dstream = aligned(dy), aligned(dstream)
-        dx = torch.empty_like(x)
-        dw = scratch = None
-        if ctx.needs_input_grad[2]:
-            dw = torch.empty_like(weight)
-            nbytes = _lib.load().jla_rms_norm_bwd_scratch_bytes(rows, dim)
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _lib.launch("jla_rms_norm_bwd", x.device, _DTYPES[x.dtype], rows, dim, _ptr(x),
-                    None if residual is None else _ptr(residual), _ptr(rstd), _ptr(weight), _ptr(dy),
-                    None if dstream is None else _ptr(dstream), _ptr(dx), None if dw is None else _ptr(dw),
-                    None if scratch is None else _ptr(scratch), 0 if scratch is None else scratch.numel())
-        return dx, dx if ctx.needs_input_grad[1] else None, dw, None
-
-
-def _rms_norm_fwd(x, residual, weight, eps, e4m3, keep_rstd):
-    dim, device = x.shape[-1], x.device
-    rows = x.numel() // dim
-    y = torch.empty_like(x, dtype=torch.float8_e4m3fn) if e4m3 else torch.empty_like(x)
-    stream = None if residual is None else torch.empty_like(x)
-    rstd = torch.empty(rows, dtype=torch.float32, device=device) if keep_rstd else None
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=device) if e4m3 else None
-    _lib.launch("jla_rms_norm_fwd", device, _DTYPES[x.dtype], rows, dim, x.data_ptr(),
-                None if residual is None else residual.data_ptr(), weight.data_ptr(), eps, e4m3, y.data_ptr(),
-                None if stream is None else stream.data_ptr(), None if rstd is None else rstd.data_ptr(),
-                None if scale is None else scale.data_ptr())
-    return y, stream, rstd, scale
-
-
 def rms_norm(x, weight, *, residual=None, eps: float = 1e-6, out_dtype=None):
     """``y = t * rsqrt(mean(t^2) + eps) * weight`` over the last axis with ``t = x`` or ``x + residual``.
 
@@ -138,28 +89,21 @@ def rms_norm(x, weight, *, residual=None, eps: float = 1e-6, out_dtype=None):
     the row's largest ``|y|`` over 448 (1 for a row of zeros), ``q * scale`` stands for ``y``. That form has no gradient and is
     refused where one would be recorded.
     """
+    out = (_lib._torch_ops or _lib.torch_ops()).rms_norm(x, weight, residual, eps, out_dtype)
+    if out is not None:
+        return out
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("rms_norm runs on CUDA tensors only: the 'cuda' implementation has no CPU fallback")
     if x.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {x.dtype}")
     if x.ndim < 1 or not 1 <= x.shape[-1] <= 16384:
         raise ValueError(f"x must be [..., dim] with 1 <= dim <= 16384; got {tuple(x.shape)}")
-    if weight.shape != x.shape[-1:] or weight.device != x.device:
-        raise ValueError(f"weight must be [{x.shape[-1]}] on {x.device}; got {tuple(weight.shape)} on {weight.device}")
+    if not isinstance(weight, torch.Tensor) or weight.shape != x.shape[-1:] or weight.device != x.device or not weight.is_floating_point():
+        raise ValueError(f"weight must be a floating [{x.shape[-1]}] on {x.device}; got "
+                         f"{weight if not isinstance(weight, torch.Tensor) else (weight.dtype, tuple(weight.shape), weight.device)}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError(f"residual must be {x.dtype} {tuple(x.shape)} on {x.device}; got {residual.dtype} "
                          f"{tuple(residual.shape)} on {residual.device}")
-    e4m3 = out_dtype == torch.float8_e4m3fn
-    if out_dtype is not None and not e4m3 and out_dtype != x.dtype:
+    if out_dtype not in (None, x.dtype, torch.float8_e4m3fn):
         raise ValueError(f"out_dtype must be {x.dtype} or torch.float8_e4m3fn; got {out_dtype}")
-    plain = nothing_to_differentiate((x, weight, residual))
-    if e4m3 and not plain:
-        raise ValueError("an e4m3 output has no gradient: call rms_norm under torch.no_grad(), or with out_dtype=None")
-    x, weight, residual = aligned(x), aligned(weight if weight.dtype is torch.float32 else weight.float()), aligned(residual)
-    if plain:
-        y, stream, _, scale = _rms_norm_fwd(x, residual, weight, float(eps), e4m3, False)
-    else:
-        (y, stream), scale = _RMSNorm.apply(x, residual, weight, float(eps)), None
-    out = (y,) if scale is None else (y, scale)
-    out = out if stream is None else (*out, stream)
-    return out[0] if len(out) == 1 else out
+    raise ValueError("an e4m3 output has no gradient: call rms_norm under torch.no_grad(), or with out_dtype=None")

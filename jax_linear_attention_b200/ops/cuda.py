@@ -61,14 +61,6 @@ def cast(x, dtype, device=None):
     return x.to(device=device, dtype=dtype).contiguous()
 
 
-def aligned(x):
-    """``x`` contiguous and on a 16-byte boundary (a slice of another tensor may start anywhere); None stays None."""
-    if x is None or (x.is_contiguous() and not x.data_ptr() & 15):
-        return x
-    x = x.contiguous()
-    return x.clone() if x.data_ptr() & 15 else x
-
-
 VALUE_BLOCK = 128  # value channels per head of the chunk kernels
 
 
