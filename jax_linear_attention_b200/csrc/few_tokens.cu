@@ -43,8 +43,8 @@ template <int BN, bool GATED> struct Shape {
   // Partial sums that arrive: whole rounds of up to eight parts, [weight][part][token][128 features].
   static constexpr int kPartRows = BN + kMaxSplit, kPartBytes = kWeights * kPartRows * 512;
   // The ring of operand tiles; afterwards this CTA's own partial sums, [weight][token][128 features]. Two CTAs share an SM
-  // where the sums leave room for that: twice as many clusters fit the GPU.
-  static constexpr int kCtas = kWeights * BN <= 32 ? 2 : 1;
+  // where one weight's sums leave room for that: twice as many clusters fit the GPU.
+  static constexpr int kCtas = !GATED && BN <= 32 ? 2 : 1;
   static constexpr int kRoom = (kCtas == 2 ? 110 : 224) * 1024 - 1024 - kPartBytes;
   static constexpr int kFit = kRoom / kStageBytes;
   static constexpr int kStages = kFit < 12 ? kFit : 12;

@@ -43,8 +43,8 @@ const char* fwd_problem(int dtype, int out_dtype, int64_t rows, int in, int out,
   if (!e4m3 && dtype != JLA_DTYPE_BF16 && dtype != JLA_DTYPE_F16) return "linear: operands must be bf16, f16 or e4m3";
   if (out_dtype != JLA_DTYPE_BF16 && out_dtype != JLA_DTYPE_F16) return "linear: the output must be bf16 or f16";
   if (!e4m3 && out_dtype != dtype) return "linear: the output has the operands' type unless they are e4m3";
-  if (e4m3 != (x_scale != nullptr) || e4m3 != (w_scale != nullptr) || e4m3 != (w_scale2 != nullptr)) {
-    return "linear: scales go with e4m3 operands";
+  if (rows != 0 && (e4m3 != (x_scale != nullptr) || e4m3 != (w_scale != nullptr) || e4m3 != (w_scale2 != nullptr))) {
+    return "linear: scales go with e4m3 operands";  // (those of no rows may be a null pointer)
   }
   if (act < JLA_ACT_NONE || act > JLA_ACT_SIGMOID) return "linear: unknown activation";
   if (const char* why = sizes_problem(rows, in, out, e4m3 ? 16 : 8)) return why;

@@ -81,10 +81,10 @@ const float* fptr(const Tensor& t) { return static_cast<const float*>(ptr(t)); }
 float* fmut(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 jla_stream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
-// Contiguous and on a 16-byte boundary (a slice of another tensor may start anywhere).
+// Contiguous, no lazily negated view, and on a 16-byte boundary (a slice of another tensor may start anywhere).
 Tensor aligned(const Tensor& t) {
   if (!t.defined()) return t;
-  Tensor c = t.contiguous();
+  Tensor c = t.contiguous().resolve_neg();
   return reinterpret_cast<uintptr_t>(c.data_ptr()) & 15 ? c.clone() : c;
 }
 
@@ -95,7 +95,7 @@ struct Rows {
 };
 Rows rows_of(const Tensor& x, int64_t width) {
   const int64_t rows = x.numel() / width, last = x.dim() - 1;
-  if (!x.is_contiguous() && x.stride(last) == 1) {
+  if (!x.is_contiguous() && x.stride(last) == 1 && !x.is_neg()) {
     int64_t stride = -1, next = 0;
     bool even = true;
     for (int64_t i = last - 1; i >= 0 && even; --i) {
@@ -127,7 +127,7 @@ variable_list once(variable_list grads) {
   for (Tensor& g : grads) {
     if (!g.defined()) continue;
     auto error = std::make_shared<torch::autograd::DelayedError>("the gradients of this operator cannot be differentiated again", 1);
-    g = (*error)(variable_list{g})[0];
+    g = (*error)(variable_list{g.detach().requires_grad_(true)})[0];
   }
   return grads;
 }

@@ -306,6 +306,10 @@ def test_no_rows():
     h = layers.gated_linear(x, w, up)
     for g in torch.autograd.grad(h.sum(), [x, w, up]):
         assert not bool(g.any())
+    q, s = torch.zeros(0, 64, device="cuda").to(torch.float8_e4m3fn), torch.zeros(0, device="cuda")
+    qw, sw = _e4m3(t["w"].detach().float())
+    assert layers.linear(q, qw, x_scale=s, weight_scale=sw).shape == (0, 72)
+    assert layers.gated_linear(q, qw, qw, x_scale=s, gate_scale=sw, up_scale=sw).shape == (0, 72)
 
 
 def test_what_lies_behind_the_rows_is_left_alone():
