@@ -81,11 +81,15 @@ __device__ __forceinline__ void finish(const Params& p, int token, int f, Quad v
 #pragma unroll
   for (int i = 0; i < 4; ++i) v.v[i] = activate<ACT>(v.v[i]) * (GATED ? u.v[i] : 1.f);
   if (!GATED && p.residual) {
-    const float2 lo = unpack_out(p.half, res.x), hi = unpack_out(p.half, res.y);
-    v.v[0] += lo.x, v.v[1] += lo.y, v.v[2] += hi.x, v.v[3] += hi.y;
+    with_half(p.half, [&](auto is_half) {
+      const float2 lo = unpack_out<is_half()>(res.x), hi = unpack_out<is_half()>(res.y);
+      v.v[0] += lo.x, v.v[1] += lo.y, v.v[2] += hi.x, v.v[3] += hi.y;
+    });
   }
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at) =
-      make_uint2(pack_out(p.half, v.v[0], v.v[1]), pack_out(p.half, v.v[2], v.v[3]));
+  with_half(p.half, [&](auto is_half) {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at) =
+        make_uint2(pack_out<is_half()>(v.v[0], v.v[1]), pack_out<is_half()>(v.v[2], v.v[3]));
+  });
 }
 
 template <int BN, bool W_MN, bool FP8, bool GATED>

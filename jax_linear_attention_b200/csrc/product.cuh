@@ -48,18 +48,27 @@ __device__ __forceinline__ float activation_slope(float z) {
   return ACT == kActSigmoid ? s * (1.f - s) : s * (1.f + z * (1.f - s));
 }
 
-// Two float32 values rounded to bf16 or f16 (`half`) in one register.
-__device__ __forceinline__ uint32_t pack_out(bool half, float lo, float hi) {
-  if (half) {
+// f(std::true_type) for float16 outputs, f(std::false_type) for bfloat16
+template <typename F>
+__device__ __forceinline__ void with_half(bool half, F&& f) {
+  if (half) f(std::true_type{});
+  else f(std::false_type{});
+}
+
+// Two float32 values rounded to bf16 or f16 (HALF) in one register.
+template <bool HALF>
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
+  if constexpr (HALF) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float2 unpack_out(bool half, uint32_t x) {
-  return half ? __half22float2(*reinterpret_cast<const __half2*>(&x))
-              : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+template <bool HALF>
+__device__ __forceinline__ float2 unpack_out(uint32_t x) {
+  if constexpr (HALF) return __half22float2(*reinterpret_cast<const __half2*>(&x));
+  else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
 }
 
 // One product (host view). "tokens" are the rows of y, "features" its columns; the contraction runs over `depth`, and over

@@ -152,7 +152,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     // ---- loads: this CTA's 128 rows of x and its half of the weight's; the bytes count on the leader's barrier
     if (lane == 0) {
       tma::prefetch_map(&maps.x[0]);
-      tma::prefetch_map(&maps.w[0]);
+      tma::prefetch_map(&maps.w[GATED ? rank : 0]);
     }
     const uint32_t bars = umma::map_rank(smem_addr(full), 0), mine = smem_addr(full), freed = smem_addr(empty);
     int s = 0, issued = 0;
@@ -308,20 +308,24 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
               for (int i = 0; i < 32; ++i) v[i] = activate<act()>(v[i]);
             });
             if (p.residual) {
+              with_half(half, [&](auto is_half) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint4 q = res[4 * h + j];
-                const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+                for (int j = 0; j < 4; ++j) {
+                  const uint4 q = res[4 * h + j];
+                  const uint32_t e[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float2 f = unpack_out(half, e[i]);
-                  v[8 * j + 2 * i] += f.x, v[8 * j + 2 * i + 1] += f.y;
+                  for (int i = 0; i < 4; ++i) {
+                    const float2 f = unpack_out<is_half()>(e[i]);
+                    v[8 * j + 2 * i] += f.x, v[8 * j + 2 * i + 1] += f.y;
+                  }
                 }
-              }
+              });
             }
           }
+          with_half(half, [&](auto is_half) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) out[16 * h + i] = pack_out(half, v[2 * i], v[2 * i + 1]);
+            for (int i = 0; i < 16; ++i) out[16 * h + i] = pack_out<is_half()>(v[2 * i], v[2 * i + 1]);
+          });
         }
         stage.store64(out, lane, &maps.y[g], col, row0, p.features, p.rows);
       }
