@@ -10,6 +10,7 @@
 // A thread owns eight adjacent columns and walks rows, so that dbias is summed in registers, over the block's eight row
 // lanes in shared memory, and over the blocks by column_sums(): the same order every time.
 #include "column_sums.cuh"
+#include "overlap.cuh"
 #include "product.cuh"
 #include "profile.cuh"
 
@@ -29,13 +30,13 @@ struct ActParams {
 
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint4 q = *(reinterpret_cast<const uint4*>(p));
   const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = to_f32(e[i]);
 }
 __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  const float4 a = *(reinterpret_cast<const float4*>(p)), b = *(reinterpret_cast<const float4*>(p) + 1);
   f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
 }
 template <typename T>
@@ -53,6 +54,8 @@ __global__ void __launch_bounds__(kColLanes * kRowLanes) activation_bwd_kernel(A
   const int col = (blockIdx.x * kColLanes + ct) * 8;
   const bool on = col < p.cols;
   float sum[8] = {};
+  start_next();
+  wait_for_previous();
   for (long r = (long)blockIdx.y * kRowLanes + lr; r < p.rows; r += (long)gridDim.y * kRowLanes) {
     if (!on) break;
     const size_t at = (size_t)r * p.cols + col;
@@ -154,10 +157,9 @@ int jla_activation_bwd(int dtype, int64_t rows, int out, int act, const float* z
   const dim3 grid = grid_of(rows, out);
   {
     ProfScope scope(kProfActBwd, s);
-    if (dtype == JLA_DTYPE_BF16) activation_bwd_kernel<__nv_bfloat16, false><<<grid, kColLanes * kRowLanes, 0, s>>>(p);
-    else activation_bwd_kernel<__half, false><<<grid, kColLanes * kRowLanes, 0, s>>>(p);
+    auto* kern = dtype == JLA_DTYPE_BF16 ? activation_bwd_kernel<__nv_bfloat16, false> : activation_bwd_kernel<__half, false>;
+    JLA_CUDA_OK(launch_overlapped(kern, grid, dim3(kColLanes * kRowLanes), 0, s, 0, p));
   }
-  JLA_LAUNCH_OK();
   return dbias ? column_sums(p.partial, grid.y, out, dbias, s) : JLA_OK;
 }
 
@@ -178,10 +180,9 @@ int jla_gated_activation_bwd(int dtype, int64_t rows, int out, int act, const fl
   const dim3 grid = grid_of(rows, out);
   {
     ProfScope scope(kProfActBwd, s);
-    if (dtype == JLA_DTYPE_BF16) activation_bwd_kernel<__nv_bfloat16, true><<<grid, kColLanes * kRowLanes, 0, s>>>(p);
-    else activation_bwd_kernel<__half, true><<<grid, kColLanes * kRowLanes, 0, s>>>(p);
+    auto* kern = dtype == JLA_DTYPE_BF16 ? activation_bwd_kernel<__nv_bfloat16, true> : activation_bwd_kernel<__half, true>;
+    JLA_CUDA_OK(launch_overlapped(kern, grid, dim3(kColLanes * kRowLanes), 0, s, 0, p));
   }
-  JLA_LAUNCH_OK();
   return JLA_OK;
 }
 

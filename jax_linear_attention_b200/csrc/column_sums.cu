@@ -1,16 +1,19 @@
 #include "column_sums.cuh"
 
+#include "overlap.cuh"
+
 namespace jla {
 namespace {
 
 // A block adds up 32 columns: lane = column (128 contiguous bytes of a partial row), warp w takes the rows w, w + 32, ...
 // and the 32 warps' sums are joined by a tree over shared memory.
-__global__ void __launch_bounds__(1024) column_sums_kernel(const float* __restrict__ partial, int parts, int cols,
-                                                           float* __restrict__ out) {
+__global__ void __launch_bounds__(1024) column_sums_kernel(const float* partial, int parts, int cols, float* out) {
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float sum = 0.f;
+  start_next();
+  wait_for_previous();
   if (c < cols) {
     for (int p = warp; p < parts; p += 32) sum += partial[(size_t)p * cols + c];
   }
@@ -27,8 +30,7 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const float* __restri
 
 int column_sums(const float* partial, int parts, int cols, float* out, cudaStream_t stream) {
   if (cols <= 0) return JLA_OK;
-  column_sums_kernel<<<(cols + 31) / 32, 1024, 0, stream>>>(partial, parts, cols, out);
-  JLA_LAUNCH_OK();
+  JLA_CUDA_OK(launch_overlapped(column_sums_kernel, dim3((cols + 31) / 32), dim3(1024), 0, stream, 0, partial, parts, cols, out));
   return JLA_OK;
 }
 

@@ -8,6 +8,7 @@
 // shared memory, and add the parts up in the order of the parts, every time the same.
 //
 // Every wait is bounded, as in product_tc.cu (kStatusFewTokens).
+#include "overlap.cuh"
 #include "product.cuh"
 #include "profile.cuh"
 #include "umma_pair.cuh"
@@ -61,7 +62,7 @@ struct Quad {
 };
 __device__ __forceinline__ Quad quad(const float* p) {
   if (!p) return Quad{};
-  const float4 f = __ldg(reinterpret_cast<const float4*>(p));
+  const float4 f = *(reinterpret_cast<const float4*>(p));
   return Quad{{f.x, f.y, f.z, f.w}};
 }
 
@@ -150,12 +151,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_token
   umma::cluster_arrive();  // (waited for before the first partial sums leave for another CTA)
   if (warp == 4) {  // the first copies wait for nobody
     asm volatile("bar.arrive 1, %0;\n" ::"n"(kThreads) : "memory");
+    wait_for_previous();
     if (umma::elect_one()) {
       for (int it = 0; it < asked; ++it) load(it, it);
     }
     __syncwarp();
   } else {
     asm volatile("bar.sync 1, %0;\n" ::"n"(kThreads) : "memory");
+    start_next();
+    wait_for_previous();
   }
   umma::fence_after_sync();
   const uint32_t tmem = tmem_slot;
@@ -274,9 +278,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_token
           const int c = min(c0 + b * kWarps, mine - 1), token = m0 + part * per + c;
           at[b] = from + c * 512;
           xs[b] = 1.f, res[b] = make_uint2(0, 0);
-          if constexpr (FP8) xs[b] = __ldg(p.x_scale + token);
+          if constexpr (FP8) xs[b] = *(p.x_scale + token);
           if (!GATED && p.residual) {
-            res[b] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + (size_t)token * p.features + f4));
+            res[b] = *(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + (size_t)token * p.features + f4));
           }
 #pragma unroll
           for (int i = 0; i < NW; ++i) sum[b][i] = Quad{};
@@ -342,12 +346,6 @@ int launch(const Product& p, int device, int sms, cudaStream_t s) {
   auto* kern = few_tokens_kernel<BN, W_MN, FP8, GATED>;
   static std::atomic<uint64_t> allowed{0};
   JLA_CUDA_OK(allow_smem(kern, S::kSmem, device, allowed));
-  cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr, cfg.numAttrs = 1;
   // Parts of the contraction: as many as there is room for at one time, each of at least two steps. (A cluster lies within
   // one of the GPU's groups of SMs, so fewer large clusters fit than their CTAs' number says; one that had to wait for
   // another to finish would double the time.)
@@ -357,8 +355,12 @@ int launch(const Product& p, int device, int sms, cudaStream_t s) {
     if (c * 2 > q.kt || device >= 64) continue;
     int fit = room[device][c].load(std::memory_order_relaxed);
     if (fit == 0) {
-      attr.val.clusterDim.x = c;
-      cfg.gridDim = dim3(c);
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(c), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = s;
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = c, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr, cfg.numAttrs = 1;
       JLA_CUDA_OK(cudaOccupancyMaxActiveClusters(&fit, kern, &cfg));
       room[device][c].store(fit > 0 ? fit : -1, std::memory_order_relaxed);
     }
@@ -367,13 +369,8 @@ int launch(const Product& p, int device, int sms, cudaStream_t s) {
       break;
     }
   }
-  cfg.gridDim = dim3(tiles_f * split, tiles_m);
-  attr.val.clusterDim.x = split;
-  {
-    ProfScope scope(kProfFewTokens, s);
-    JLA_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, maps, q, split));
-  }
-  JLA_LAUNCH_OK();
+  ProfScope scope(kProfFewTokens, s);
+  JLA_CUDA_OK(launch_overlapped(kern, dim3(tiles_f * split, tiles_m), dim3(kThreads), S::kSmem, s, split, maps, q, split));
   return JLA_OK;
 }
 

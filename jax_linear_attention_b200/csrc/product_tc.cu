@@ -14,6 +14,7 @@
 // Where the operands end inside a tile TMA reads zeros and its stores leave out what lies beyond. No load is multicast.
 // Every wait is bounded: one that runs out records kStatusProduct, and the kernel lets its copies and products in flight
 // finish, frees its TMEM and returns.
+#include "overlap.cuh"
 #include "product.cuh"
 #include "profile.cuh"
 #include "umma_pair.cuh"
@@ -108,7 +109,7 @@ struct Columns {
   float v[2];
   __device__ __forceinline__ void read(const float* p, int col, int lane, int cols) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) v[h] = p && col + 32 * h + lane < cols ? __ldg(p + col + 32 * h + lane) : 0.f;
+    for (int h = 0; h < 2; ++h) v[h] = p && col + 32 * h + lane < cols ? *(p + col + 32 * h + lane) : 0.f;
   }
   __device__ __forceinline__ float at(int h, int i) const { return __shfl_sync(0xffffffffu, v[h], i); }
 };
@@ -145,6 +146,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
   umma::fence_after_sync();
   const uint32_t tmem = tmem_slot;
   bool ok = true;
+  start_next();
+  wait_for_previous();
 
   if (warp == 0) {
     // ---- loads: this CTA's 128 rows of x and its half of the weight's; the bytes count on the leader's barrier
@@ -254,12 +257,12 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         if constexpr (!GATED) {
           const uint4* r = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + (size_t)row * p.features + col);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) res[j] = live && col + 8 * j < p.features ? __ldg(r + j) : make_uint4(0, 0, 0, 0);
+          for (int j = 0; j < 8; ++j) res[j] = live && col + 8 * j < p.features ? *(r + j) : make_uint4(0, 0, 0, 0);
         }
       };
       if (!GATED && p.residual) read_residual(tn * COLS + odd * 64);
       float xs = 1.f;
-      if constexpr (FP8) xs = live ? __ldg(p.x_scale + row) : 0.f;
+      if constexpr (FP8) xs = live ? *(p.x_scale + row) : 0.f;
       ok = umma::mbar_wait(acc_full + a, (n >> 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
@@ -382,11 +385,8 @@ int launch(const Product& p, int device, int sms, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   JLA_CUDA_OK(allow_smem(kern, S::kSmem, device, allowed));
   const int pairs = sms / 2 < q.tiles ? sms / 2 : q.tiles;
-  {
-    ProfScope scope(kProfProduct, s);
-    kern<<<2 * pairs, kThreads, S::kSmem, s>>>(maps, q);
-  }
-  JLA_LAUNCH_OK();
+  ProfScope scope(kProfProduct, s);
+  JLA_CUDA_OK(launch_overlapped(kern, dim3(2 * pairs), dim3(kThreads), S::kSmem, s, 0, maps, q));  // (the kernel has its cluster size)
   return JLA_OK;
 }
 

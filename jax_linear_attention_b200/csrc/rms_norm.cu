@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "column_sums.cuh"
+#include "overlap.cuh"
 #include "profile.cuh"
 
 namespace jla {
@@ -98,11 +99,11 @@ template <typename T, int VEC> struct Raw {
 template <int VEC>
 __device__ __forceinline__ void load_weight(const float* p, float (&f)[VEC]) {
   if constexpr (VEC == 1) {
-    f[0] = __ldg(p);
+    f[0] = *(p);
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; i += 4) {
-      const float4 u = __ldg(reinterpret_cast<const float4*>(p + i));
+      const float4 u = *(reinterpret_cast<const float4*>(p + i));
       f[i] = u.x, f[i + 1] = u.y, f[i + 2] = u.z, f[i + 3] = u.w;
     }
   }
@@ -204,6 +205,8 @@ __global__ void __launch_bounds__(1024) rms_norm_fwd_kernel(RmsParams p) {
   const T* x = static_cast<const T*>(p.x);
   const T* res = static_cast<const T*>(p.residual);
   R xr[VPT], rr[VPT];
+  start_next();
+  wait_for_previous();
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int c = (j * tpr + threadIdx.x) * VEC;
@@ -317,6 +320,8 @@ __global__ void __launch_bounds__(MAXT) rms_norm_bwd_kernel(RmsParams p) {
     }
     rstd_next = live ? p.rstd[row] : 0.f;
   };
+  start_next();
+  wait_for_previous();
   const long first = (long)blockIdx.x * blockDim.y, step = (long)gridDim.x * blockDim.y;
   if (kAhead && first < p.rows) request(first);
   int turn = 0;
@@ -418,7 +423,8 @@ RowShape row_shape(int vectors, int vpt) {
 }
 
 template <typename T, bool E4M3>
-void launch_fwd(const RmsParams& p, bool vec, cudaStream_t s) {
+cudaError_t launch_fwd(const RmsParams& p, bool vec, cudaStream_t s) {
+  cudaError_t err = cudaSuccess;
   // Few rows: one vector a thread, so that a row's loads all leave at once (a decoding step is latency). Many rows: four
   // vectors, fewer threads meet in the reduction and more rows are in flight.
   constexpr int VEC = 16 / sizeof(T);
@@ -426,12 +432,13 @@ void launch_fwd(const RmsParams& p, bool vec, cudaStream_t s) {
   const RowShape b = row_shape(vectors, vec ? (vectors <= 1024 && p.rows <= 148 ? 1 : 4) : (vectors <= 4096 ? 4 : 16));
   const dim3 block(b.tpr, b.rpb), grid((unsigned)((p.rows + b.rpb - 1) / b.rpb));
   if (vec) {
-    if (b.vpt == 1) rms_norm_fwd_kernel<T, VEC, 1, E4M3><<<grid, block, 0, s>>>(p);
-    else rms_norm_fwd_kernel<T, VEC, 4, E4M3><<<grid, block, 0, s>>>(p);
+    if (b.vpt == 1) err = launch_overlapped(rms_norm_fwd_kernel<T, VEC, 1, E4M3>, grid, block, 0, s, 0, p);
+    else err = launch_overlapped(rms_norm_fwd_kernel<T, VEC, 4, E4M3>, grid, block, 0, s, 0, p);
   } else {
-    if (b.vpt == 4) rms_norm_fwd_kernel<T, 1, 4, E4M3><<<grid, block, 0, s>>>(p);
-    else rms_norm_fwd_kernel<T, 1, 16, E4M3><<<grid, block, 0, s>>>(p);
+    if (b.vpt == 4) err = launch_overlapped(rms_norm_fwd_kernel<T, 1, 4, E4M3>, grid, block, 0, s, 0, p);
+    else err = launch_overlapped(rms_norm_fwd_kernel<T, 1, 16, E4M3>, grid, block, 0, s, 0, p);
   }
+  return err;
 }
 
 // Backward: two vectors a thread (registers), four where a block would not have the threads.
@@ -446,23 +453,25 @@ int bwd_blocks(long rows, const RowShape& b) {
 }
 
 template <typename T>
-void launch_bwd(const RmsParams& p, const RowShape& b, int blocks, bool vec, cudaStream_t s) {
+cudaError_t launch_bwd(const RmsParams& p, const RowShape& b, int blocks, bool vec, cudaStream_t s) {
+  cudaError_t err = cudaSuccess;
   constexpr int VEC = 16 / sizeof(T);
   const dim3 block(b.tpr, b.rpb);
   const size_t smem = b.rpb > 1 && p.partial ? (size_t)b.rpb * p.dim * sizeof(float) : 0;  // at most 16 KB
   if (vec && b.vpt == 2) {
-    if (b.tpr > 512) rms_norm_bwd_kernel<T, VEC, 2, 1024><<<blocks, block, smem, s>>>(p);
-    else if (b.tpr > 256) rms_norm_bwd_kernel<T, VEC, 2, 512><<<blocks, block, smem, s>>>(p);
-    else rms_norm_bwd_kernel<T, VEC, 2, 256><<<blocks, block, smem, s>>>(p);
+    if (b.tpr > 512) err = launch_overlapped(rms_norm_bwd_kernel<T, VEC, 2, 1024>, dim3(blocks), block, smem, s, 0, p);
+    else if (b.tpr > 256) err = launch_overlapped(rms_norm_bwd_kernel<T, VEC, 2, 512>, dim3(blocks), block, smem, s, 0, p);
+    else err = launch_overlapped(rms_norm_bwd_kernel<T, VEC, 2, 256>, dim3(blocks), block, smem, s, 0, p);
   } else if (vec) {
-    if constexpr (VEC == 4) rms_norm_bwd_kernel<T, VEC, 4, 1024><<<blocks, block, smem, s>>>(p);
+    if constexpr (VEC == 4) err = launch_overlapped(rms_norm_bwd_kernel<T, VEC, 4, 1024>, dim3(blocks), block, smem, s, 0, p);
   } else if (b.vpt == 4) {
-    if (b.tpr > 512) rms_norm_bwd_kernel<T, 1, 4, 1024><<<blocks, block, smem, s>>>(p);
-    else if (b.tpr > 256) rms_norm_bwd_kernel<T, 1, 4, 512><<<blocks, block, smem, s>>>(p);
-    else rms_norm_bwd_kernel<T, 1, 4, 256><<<blocks, block, smem, s>>>(p);
+    if (b.tpr > 512) err = launch_overlapped(rms_norm_bwd_kernel<T, 1, 4, 1024>, dim3(blocks), block, smem, s, 0, p);
+    else if (b.tpr > 256) err = launch_overlapped(rms_norm_bwd_kernel<T, 1, 4, 512>, dim3(blocks), block, smem, s, 0, p);
+    else err = launch_overlapped(rms_norm_bwd_kernel<T, 1, 4, 256>, dim3(blocks), block, smem, s, 0, p);
   } else {
-    rms_norm_bwd_kernel<T, 1, 16, 1024><<<blocks, block, smem, s>>>(p);
+    err = launch_overlapped(rms_norm_bwd_kernel<T, 1, 16, 1024>, dim3(blocks), block, smem, s, 0, p);
   }
+  return err;
 }
 
 }  // namespace
@@ -489,15 +498,16 @@ int jla_rms_norm_fwd(int dtype, int64_t rows, int dim, const void* x, const void
   const bool vec = dim % (dtype == JLA_DTYPE_F32 ? 4 : 8) == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) &&
                    aligned16(y) && aligned16(stream_out);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t err = cudaSuccess;
   {
     ProfScope scope(kProfRmsNorm, s);
     switch (dtype) {
-      case JLA_DTYPE_BF16: out_e4m3 ? launch_fwd<__nv_bfloat16, true>(p, vec, s) : launch_fwd<__nv_bfloat16, false>(p, vec, s); break;
-      case JLA_DTYPE_F16: out_e4m3 ? launch_fwd<__half, true>(p, vec, s) : launch_fwd<__half, false>(p, vec, s); break;
-      default: out_e4m3 ? launch_fwd<float, true>(p, vec, s) : launch_fwd<float, false>(p, vec, s); break;
+      case JLA_DTYPE_BF16: err = out_e4m3 ? launch_fwd<__nv_bfloat16, true>(p, vec, s) : launch_fwd<__nv_bfloat16, false>(p, vec, s); break;
+      case JLA_DTYPE_F16: err = out_e4m3 ? launch_fwd<__half, true>(p, vec, s) : launch_fwd<__half, false>(p, vec, s); break;
+      default: err = out_e4m3 ? launch_fwd<float, true>(p, vec, s) : launch_fwd<float, false>(p, vec, s); break;
     }
   }
-  JLA_LAUNCH_OK();
+  JLA_CUDA_OK(err);
   return JLA_OK;
 }
 
@@ -540,15 +550,16 @@ int jla_rms_norm_bwd(int dtype, int64_t rows, int dim, const void* x, const void
                    aligned16(dstream) && aligned16(dx);
   const RowShape b = bwd_shape(dim, vec ? width : 1);
   const int blocks = bwd_blocks(rows, b);
+  cudaError_t err = cudaSuccess;
   {
     ProfScope scope(kProfRmsNormBwd, s);
     switch (dtype) {
-      case JLA_DTYPE_BF16: launch_bwd<__nv_bfloat16>(p, b, blocks, vec, s); break;
-      case JLA_DTYPE_F16: launch_bwd<__half>(p, b, blocks, vec, s); break;
-      default: launch_bwd<float>(p, b, blocks, vec, s); break;
+      case JLA_DTYPE_BF16: err = launch_bwd<__nv_bfloat16>(p, b, blocks, vec, s); break;
+      case JLA_DTYPE_F16: err = launch_bwd<__half>(p, b, blocks, vec, s); break;
+      default: err = launch_bwd<float>(p, b, blocks, vec, s); break;
     }
   }
-  JLA_LAUNCH_OK();
+  JLA_CUDA_OK(err);
   return dweight ? column_sums(p.partial, blocks, dim, dweight, s) : JLA_OK;
 }
 

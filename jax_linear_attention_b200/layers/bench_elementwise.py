@@ -1,5 +1,6 @@
 """Device times of the element-wise layer kernels around the op, forward and backward, at the shapes of the benchmark
-workloads: ``python -m jax_linear_attention_b200.layers.bench_elementwise [--only gates|conv|norm] [--steps N]``.
+workloads: ``python -m jax_linear_attention_b200.layers.bench_elementwise [--only gates|conv|norm|stream|product] [--steps N]``;
+and of the norm of the residual stream and the matrix products around a mixer.
 
 Each case builds its tensors on the device, calls the layer function and its backward ``--warmup`` times and then
 ``--steps`` times between CUDA events, writing a buffer larger than L2 before every call so that the inputs come from
@@ -13,7 +14,7 @@ import argparse
 
 import torch
 
-from . import gate_prologue, gated_rms_norm, short_conv
+from . import gate_prologue, gated_linear, gated_rms_norm, linear, rms_norm, short_conv
 
 
 def _timed(fwd, bwd, steps, warmup, flush):
@@ -68,11 +69,24 @@ def cases(dev):
                lambda o=o, z=z, wn=wn, nbg=nbg, group=group: gated_rms_norm(o, z, wn, norm_before_gate=nbg, group_size=group),
                lambda y, o=o, z=z, wn=wn, dyn=dyn: torch.autograd.grad([y], [o, z, wn], [dyn]),
                (o.numel() * 6, o.numel() * 10))
+    # residual stream in front of a mixer, and the projections and feed-forward block of a model 2048 wide
+    x = torch.randn(16384, 2048, device=dev, dtype=bf16, requires_grad=True)
+    r = torch.randn(16384, 2048, device=dev, dtype=bf16, requires_grad=True)
+    ws, dys = torch.ones(2048, device=dev, requires_grad=True), torch.randn(16384, 2048, device=dev, dtype=bf16)
+    yield ("stream", "RMS norm with residual 16384 x 2048", lambda: rms_norm(x, ws, residual=r),
+           lambda out: torch.autograd.grad(list(out), [x, r, ws], [dys, dys]), (x.numel() * 8, x.numel() * 10))
+    wo = (torch.randn(2048, 2048, device=dev) / 45).to(bf16).requires_grad_(True)
+    yield ("product", "linear with residual 16384 x 2048 x 2048", lambda: linear(x, wo, residual=r),
+           lambda out: torch.autograd.grad(out, [x, wo, r], dys), (x.numel() * 6, x.numel() * 6))
+    wg, wu = ((torch.randn(5632, 2048, device=dev) / 45).to(bf16).requires_grad_(True) for _ in range(2))
+    dh = torch.randn(16384, 5632, device=dev, dtype=bf16)
+    yield ("product", "gated linear 16384 x 2048 x 5632", lambda: gated_linear(x, wg, wu),
+           lambda out: torch.autograd.grad(out, [x, wg, wu], dh), (x.numel() * 2 + dh.numel() * 10, dh.numel() * 14 + x.numel() * 4))
 
 
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
-    ap.add_argument("--only", choices=("gates", "conv", "norm"), default=None)
+    ap.add_argument("--only", choices=("gates", "conv", "norm", "stream", "product"), default=None)
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=3)
     args = ap.parse_args()

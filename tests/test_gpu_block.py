@@ -206,6 +206,43 @@ def test_two_streams_at_once():
         assert all(bool((p == q).all()) for p, q in zip(a, b))
 
 
+@pytest.mark.parametrize("rows", [3, 100, 2100])
+def test_kernels_that_overlap_see_what_was_written_before(rows):
+    """Blocks of a kernel start while the one before still runs: every input, weights and scales among them, is written by the
+    kernel just before, torch's or one of these."""
+    def chain(wait):
+        torch.manual_seed(5)
+        x = torch.randn(rows, 512, device="cuda").bfloat16()
+        w, up, down = ((torch.randn(512, 512, device="cuda") / 23).bfloat16() for _ in range(3))
+        n, b = torch.ones(512, device="cuda"), torch.zeros(512, device="cuda")
+        seen = []
+        for i in range(30):
+            n.add_(0.01), wait()
+            y, x = layers.rms_norm(x, n, residual=x)
+            wait(), w.mul_(0.999), wait()
+            h = layers.gated_linear(y, w, up)
+            wait(), b.add_(0.01), wait()
+            x = layers.linear(h, down, b, residual=x, activation="silu")
+            wait(), up.copy_(down), wait()
+            q, scale = layers.rms_norm(x, n, out_dtype=torch.float8_e4m3fn)
+            wait()
+            wq, ws = w.to(torch.float8_e4m3fn), torch.full((512,), 1 / (i + 1), device="cuda")
+            z = layers.linear(q, wq, x_scale=scale, weight_scale=ws)
+            wait(), x.copy_(z + x), wait()
+            seen.append(x.clone())
+        leaf = x.clone().requires_grad_()
+        y = layers.linear(layers.rms_norm(leaf, n), w, b, activation="gelu")
+        wait()
+        seen += torch.autograd.grad(y, [leaf], x)
+        return seen
+
+    def still():
+        torch.cuda.synchronize()
+
+    for a, c in zip(chain(lambda: None), chain(still)):
+        assert bool((a == c).all())
+
+
 def test_offsets_beyond_32_bits():
     rows, dim = 1_100_000, 2048  # 2.25e9 elements
     x = torch.randn(rows, dim, device="cuda", dtype=torch.bfloat16)
