@@ -385,22 +385,29 @@ int pick(const Product& p, int dev, int sms, cudaStream_t s) {
 
 }  // namespace
 
-// Up to 64 tokens always; up to 2048 where this kernel is expected to be the faster one. Measured, in us, inputs from HBM:
-//   this kernel: 8.0 + 0.34 a step of its longest CTA (gated 8.6 + 0.48)     pairs: 6.2 + 0.21 a step of the busiest pair
-//   4096 -> 256, 512 tokens: 10.7 against 18.7     4096 -> 2048, 256: 14.5, 20.2     1024 -> 1024, 256: 8.8, 9.7
-//   512 -> 4096, 128: 9.1, 8.7     2048 -> 6144, 256: 18.6, 14.8     gated 2048 -> 6144, 256: 40.9, 21.3
+// Up to 64 tokens always; up to 8192 where this kernel is expected to be the faster one. Fitted, in hundredths of a us with
+// inputs from HBM, to times of both from 33 to 1500 tokens, depths of 64 to 4096 and widths of 256 to 6144:
+//   this kernel: 200 + waves (390 + 36 a step of the longest CTA), 110 more where the contraction is split (gated 360, 48, 160)
+//   pairs: 720 + 20 a step of the busiest pair; an activation or bias shows with 290 (here 30), a residual with 200 (here 100)
+// Some of the times, in us, this kernel against pairs of CTAs: 4096 -> 256, 512 tokens: 10.7, 18.7; 4096 -> 2048, 256: 14.5,
+// 20.2; 512 -> 512, 256: 7.9, 9.6, with silu and a residual 8.4, 15.2; 2048 -> 6144, 256: 18.6, 14.8; gated 2048 -> 6144, 256:
+// 40.9, 21.3; gated 64 -> 256, 1500: 5.5, 7.6.
 bool few_tokens_applies(const Product& p, int sms) {
-  if (p.x_mn || p.group || p.rows > 2048) return false;
+  if (p.x_mn || p.group || p.rows > 8192) return false;
   if (p.rows <= 64) return true;
   const int kb = p.dtype == JLA_DTYPE_E4M3 ? 128 : 64, kt = (p.depth + kb - 1) / kb * (p.pair ? 2 : 1);
   const int bn = p.gated ? 64 : 128, tiles = (p.features + 127) / 128 * (int)((p.rows + bn - 1) / bn);
   int split = sms / tiles < kMaxSplit ? sms / tiles : kMaxSplit;
   split = split > kt / 2 ? kt / 2 : split;
   split = split < 1 ? 1 : split;
-  const int steps = (kt + split - 1) / split * ((tiles * split + sms - 1) / sms);
+  const int steps = (kt + split - 1) / split, waves = (tiles * split + sms - 1) / sms;
   const int cols = p.features * (p.gated ? 2 : 1);
   const int pair_steps = ((int)((p.rows + 255) / 256) * ((cols + 255) / 256) + sms / 2 - 1) / (sms / 2) * kt;
-  return (p.gated ? 860 + 48 * steps : 800 + 34 * steps) < 620 + 21 * pair_steps;
+  const bool busy = !p.gated && (p.act != kActNone || p.bias);
+  const int64_t here = 200 + (int64_t)waves * (p.gated ? 360 + 48 * steps : 390 + 36 * steps) + (split > 1 ? (p.gated ? 160 : 110) : 0) +
+                       (busy ? 30 : 0) + (p.residual ? 100 : 0);
+  const int64_t pairs = 720 + (int64_t)20 * pair_steps + (busy ? 290 : 0) + (p.residual ? 200 : 0);
+  return here < pairs;
 }
 
 int product_few_tokens(const Product& p, int dev, int sms, cudaStream_t s) {

@@ -159,7 +159,7 @@ def test_decoding_step_captured_and_replayed():
                 assert bool((a == b).all())
 
 
-@pytest.mark.parametrize("rows", [30, 2100])
+@pytest.mark.parametrize("rows", [30, 2100, 8300])
 def test_training_step_captured_and_replayed(rows):
     def step(x, w, up, n, b, dy):
         leaves = [x, w, up, n, b]
@@ -206,7 +206,7 @@ def test_two_streams_at_once():
         assert all(bool((p == q).all()) for p, q in zip(a, b))
 
 
-@pytest.mark.parametrize("rows", [3, 100, 2100])
+@pytest.mark.parametrize("rows", [3, 100, 2100, 8300])
 def test_kernels_that_overlap_see_what_was_written_before(rows):
     """Blocks of a kernel start while the one before still runs: every input, weights and scales among them, is written by the
     kernel just before, torch's or one of these."""

@@ -133,7 +133,7 @@ def test_linear_gradients(rows, depth, out, dtype, act, bias, residual):
 # Every kernel and tile width: few tokens (16, 32, 64 or 128 of them a block), pairs of CTAs (128 or 256 columns a tile, one
 # tile a pair and several).
 KERNELS = [(5, 2048, 136), (20, 520, 200), (50, 1000, 72), (100, 2048, 264), (100, 72, 2000), (1500, 4096, 24), (2100, 72, 56),
-           (2100, 264, 72), (2100, 136, 136), (5000, 72, 1000), (18900, 72, 256)]
+           (8300, 72, 56), (8300, 264, 72), (8300, 136, 136), (5000, 72, 1000), (2100, 520, 1000), (18900, 72, 256)]
 
 
 @pytest.mark.parametrize("rows, depth, out", KERNELS)
@@ -214,7 +214,7 @@ def _e4m3(x):
 
 @pytest.mark.parametrize("rows, depth, out", [(1, 64, 64), (1, 16, 8), (5, 2048, 136), (33, 208, 1000), (100, 4096, 72),
                                               (200, 144, 264), (300, 16, 200), (1003, 1024, 520), (18900, 80, 256),
-                                              (20, 4096, 136), (60, 4096, 136), (2100, 80, 56), (5000, 144, 1000)])
+                                              (20, 4096, 136), (60, 4096, 136), (8300, 80, 56), (8300, 80, 200), (5000, 144, 1000)])
 @pytest.mark.parametrize("out_dtype", DTYPES)
 def test_e4m3(rows, depth, out, out_dtype):
     dtype = DTYPES[out_dtype]
@@ -239,7 +239,7 @@ def test_e4m3(rows, depth, out, out_dtype):
     _close(h, want, (off + _half_step(dtype) * want.abs()) * (1 + 2.0 ** -7) + TINY)
 
 
-@pytest.mark.parametrize("rows", [12, 400])
+@pytest.mark.parametrize("rows", [12, 400, 8300])
 def test_gradients_against_differences(rows):
     t = _inputs(rows, 64, 72, torch.float16, gated=True, seed=6)
     leaves = [t[n].requires_grad_() for n in ("x", "w", "up")]
@@ -275,7 +275,7 @@ def test_shapes_strides_and_slices():
     assert bool((layers.linear(t["x"], t["w"], b, residual=t["r"]) == want).all())
 
 
-@pytest.mark.parametrize("rows", [20, 400])
+@pytest.mark.parametrize("rows", [20, 400, 8300])
 def test_gradients_of_slices_and_broadcasts(rows):
     t = _inputs(rows, 64, 72, torch.float16, gated=True)
     wide = torch.randn(rows, 200, device="cuda").half()
@@ -313,7 +313,7 @@ def test_no_rows():
 
 
 def test_what_lies_behind_the_rows_is_left_alone():
-    for rows, depth, out in ((5, 64, 72), (130, 64, 72), (300, 64, 72)):
+    for rows, depth, out in ((5, 64, 72), (130, 64, 72), (300, 64, 72), (8300, 64, 72), (8300, 64, 200)):
         t = _inputs(rows, depth, out, torch.bfloat16)
         y = layers.linear(t["x"], t["w"])
         space = torch.full((rows + 300, out), 9.0, dtype=torch.bfloat16, device="cuda")
@@ -323,7 +323,7 @@ def test_what_lies_behind_the_rows_is_left_alone():
         assert bool((space[:rows] == y).all()) and bool((space[rows:] == 9).all())
 
 
-@pytest.mark.parametrize("rows", [7, 200, 600])
+@pytest.mark.parametrize("rows", [7, 200, 600, 8300])
 def test_infinities_and_nan_stay_in_their_rows(rows):
     t = _inputs(rows, 72, 72, torch.bfloat16)
     want = layers.linear(t["x"], t["w"])
