@@ -41,6 +41,7 @@ template <int ACT>
 __device__ __forceinline__ float activation_slope(float z) {
   if constexpr (ACT == kActNone) return 1.f;
   if constexpr (ACT == kActGelu) {
+    z = fabsf(z) > 32.f ? copysignf(32.f, z) : z;  // the slope is 0 or 1 from far below that on; z^2 must not overflow (NaN stays)
     const float s = sigmoid_f32(kGelu2C * (z + kGeluA * z * z * z));
     return s + z * s * (1.f - s) * kGelu2C * (1.f + 3.f * kGeluA * z * z);
   }

@@ -334,6 +334,27 @@ def test_infinities_and_nan_stay_in_their_rows(rows):
     assert bool((got[keep] == want[keep]).all()) and bool(got[rows - 2].isnan().all()) and not bool(got[2].isfinite().any())
 
 
+@pytest.mark.parametrize("rows", [20, 8300])
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_activations_far_out(rows, act):
+    """Products up to 1e20, where exponentials and powers overflow: the activation is the identity or zero (or one), its slope
+    one or zero."""
+    x = torch.zeros(rows, 64, device="cuda", dtype=torch.bfloat16)
+    size = torch.logspace(2, 20, rows, device="cuda") * (1 - 2 * (torch.arange(rows, device="cuda") % 2))
+    x[:, 0] = size.bfloat16()
+    w = torch.zeros(72, 64, device="cuda", dtype=torch.bfloat16)
+    w[:, 0] = 1
+    x.requires_grad_(), w.requires_grad_()
+    z = x.detach().float()[:, :1].expand(rows, 72)
+    up = (z > 0).float()
+    y = layers.linear(x, w, activation=act)
+    assert bool((y.float() == (up if act == "sigmoid" else z * up)).all())
+    dx, = torch.autograd.grad(y, [x], torch.ones_like(y))
+    assert bool((dx[:, 0].float() == (0 * up[:, 0] if act == "sigmoid" else 72 * up[:, 0])).all()) and not bool(dx[:, 1:].any())
+    h = layers.gated_linear(x, w, 2.0 ** -10 * w.detach(), activation=act)
+    assert bool(h.isfinite().all() if act == "sigmoid" else (h.float()[z < 0] == 0).all())
+
+
 def test_only_what_is_asked_for():
     t = _inputs(40, 64, 72, torch.bfloat16, bias=True, gated=True)
     for name in ("x", "w", "b"):
