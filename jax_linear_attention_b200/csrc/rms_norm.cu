@@ -16,6 +16,9 @@
 // and the residual up again: the rounded stream, half the bytes to read, would leave the float32 weight gradient with an
 // error of 2e-3 instead of 2e-7.
 //
+// Measured on a B200, inputs from HBM: 16384 x 2048 bf16 with residual 44 us forward (6.0 TB/s), 60 us backward (5.6 TB/s);
+// 5003 x 4096 f16 with residual to e4m3 29 us (5.0 TB/s); one row 2.2 us.
+//
 // The weight gradient is summed in registers over the rows that a thread walks, over the block in shared memory, and
 // over the blocks by column_sums(), always in the same order.
 #include <cuda_fp8.h>
