@@ -97,7 +97,7 @@ struct Product {
 };
 
 int product_pairs(const Product& p, int device, int sms, cudaStream_t stream);       // product_tc.cu: any number of tokens
-int product_few_tokens(const Product& p, int device, int sms, cudaStream_t stream);  // few_tokens.cu: where few_tokens_applies
+int product_few_tokens(const Product& p, int device, cudaStream_t stream);  // few_tokens.cu: where few_tokens_applies
 bool few_tokens_applies(const Product& p, int sms);
 
 int* tc_status_ptr();  // status.cu

@@ -62,7 +62,7 @@ int run(const Product& p, cudaStream_t s) {
   }
   int device = 0, sms = 0;
   if (const int rc = current_device(&device, &sms)) return rc;
-  return few_tokens_applies(p, sms) ? product_few_tokens(p, device, sms, s) : product_pairs(p, device, sms, s);
+  return few_tokens_applies(p, sms) ? product_few_tokens(p, device, s) : product_pairs(p, device, sms, s);
 }
 
 }  // namespace
