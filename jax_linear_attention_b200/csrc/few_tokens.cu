@@ -407,11 +407,12 @@ bool few_tokens_applies(const Product& p, int sms) {
   split = split < 1 ? 1 : split;
   const int steps = (kt + split - 1) / split, waves = (tiles * split + sms - 1) / sms;
   const int cols = p.features * (p.gated ? 2 : 1);
-  const int pair_steps = ((int)((p.rows + 255) / 256) * ((cols + 255) / 256) + sms / 2 - 1) / (sms / 2) * kt;
+  const int pair_tiles = (int)((p.rows + 255) / 256) * ((cols + 255) / 256), rest = pair_tiles % (sms / 2);
+  const int64_t pair_rounds = pair_tiles / (sms / 2) * 100 + (rest == 0 ? 0 : 2 * rest <= sms / 2 ? 69 : 100);  // hundredths
   const bool busy = !p.gated && (p.act != kActNone || p.bias);
   const int64_t here = 200 + (int64_t)waves * (p.gated ? 360 + 48 * steps : 390 + 36 * steps) + (split > 1 ? (p.gated ? 160 : 110) : 0) +
                        (busy ? 30 : 0) + (p.residual ? 100 : 0);
-  const int64_t pairs = 720 + (int64_t)20 * pair_steps + (busy ? 290 : 0) + (p.residual ? 200 : 0);
+  const int64_t pairs = 720 + 20 * pair_rounds * kt / 100 + (busy ? 290 : 0) + (p.residual ? 200 : 0);
   return here < pairs;
 }
 

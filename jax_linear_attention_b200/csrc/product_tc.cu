@@ -10,6 +10,8 @@
 // thread of the leading CTA issues the products, eight warps of each CTA take finished accumulators out of TMEM (32 rows a
 // warp, a row a thread) through shared memory and TMA stores. Two sets of accumulators: the epilogue of one tile
 // runs under the products of the next. A pair reads an operand byte from L2 half as often as two CTAs of 128 x BN would.
+// Tiles of a last round that would leave more than half of the pairs idle are taken in halves (1003 x 2048 x 6144 f16, 96
+// tiles on 74 pairs: 31 -> 27 us with silu; 700 x 2048 x 2048, 24 tiles: 19.5 -> 15.7 us).
 //
 // Measured on a B200, inputs from HBM: 16384 x 4096 x 2048 bf16 163 us forward, 165 us dx, 177 us dW (128 tiles on 74 pairs; cuBLAS
 // 178, 169, 168); gated 16384 x 2048 x 5632 bf16 460 us, 532 us with g and u kept; gated 5003 x 2048 x 5632 e4m3 81 us. The tensor
@@ -35,13 +37,15 @@ constexpr int kStagingWarp = 4096;  // a box of 32 rows x 128 bytes for each epi
 
 struct Maps {
   CUtensorMap x[2], w[2], y[2], save[2];
+  CUtensorMap w_half[2];  // the weights in boxes of half a tile's rows (K-major)
 };
 
 struct Params {
   int rows, features;           // of y
-  int tiles_n, tiles_mn, tiles; // tiles in a row of tiles, in one product, in all
+  int tiles_n, tiles_mn;        // tiles in a row of tiles, in one product
+  int whole, pieces;            // tiles taken whole, and pieces in all: those and the halves of the others
   int kt0, kt;                  // steps of the contraction with the first pair of operands, and in all
-  uint32_t idesc;
+  uint32_t idesc, idesc_half;
   int act, half, saves;
   const float *x_scale, *w_scale[2], *bias;
   const void* residual;
@@ -65,6 +69,22 @@ __device__ __forceinline__ void locate(const Params& p, int t, int& tm, int& tn)
   tm = in / width;
   tn = band * kBand + in % width;
 }
+
+// What a pair works on at a time: a whole tile, or the left or right half of one (in a last round of tiles that would leave
+// more than half of the pairs idle; a step of half a tile takes 0.69 of the time of one of a whole tile).
+struct Piece {
+  int product, tm, tn, part;
+  bool whole;
+  template <int BN> __device__ __forceinline__ static Piece at(const Params& p, int i) {
+    Piece q;
+    q.whole = BN != 256 || i < p.whole;
+    const int t = q.whole ? i : p.whole + (i - p.whole) / 2;
+    q.part = q.whole ? 0 : (i - p.whole) % 2;
+    q.product = t / p.tiles_mn;
+    locate(p, t - q.product * p.tiles_mn, q.tm, q.tn);
+    return q;
+  }
+};
 
 // A warp's staging box: 32 rows of 128 bytes, 128-byte swizzle (16-byte chunk j of row r lies at chunk j ^ (r % 8)).
 struct Staging {
@@ -163,21 +183,21 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     const uint32_t bars = umma::map_rank(smem_addr(full), 0), mine = smem_addr(full), freed = smem_addr(empty);
     int s = 0, issued = 0;
     uint32_t phase = 1;  // (a fresh barrier's phase before the first counts as complete)
-    for (int t = first; t < p.tiles && ok; t += step) {
-      const int g = t / p.tiles_mn;
-      int tm, tn;
-      locate(p, t - g * p.tiles_mn, tm, tn);
-      const int m0 = tm * 256 + (int)rank * 128;
-      const int n0 = GATED ? tn * (BN / 2) : tn * BN + (int)rank * (BN / 2);
-      const CUtensorMap* mx = &maps.x[g];
-      const CUtensorMap* mw = &maps.w[GATED ? rank : 0];
+    for (int i = first; i < p.pieces && ok; i += step) {
+      const Piece q = Piece::at<BN>(p, i);
+      const int m0 = q.tm * 256 + (int)rank * 128;
+      const int wide = q.whole ? BN / 2 : BN / 4;  // this CTA's rows of the weight (of one of them where gated)
+      const int n0 = q.tn * (GATED ? BN / 2 : BN) + (GATED ? q.part : 2 * q.part + (int)rank) * wide;
+      const CUtensorMap* mx = &maps.x[q.product];
+      const CUtensorMap* ws_of = q.whole || W_MN ? maps.w : maps.w_half;
+      const CUtensorMap* mw = ws_of + (GATED ? rank : 0);
       int k0 = 0;
       for (int kt = 0; kt < p.kt; ++kt, k0 += FP8 ? 128 : 64) {
-        if (kt == p.kt0) mx = &maps.x[1], mw = &maps.w[1], k0 = 0;  // the second pair of operands
+        if (kt == p.kt0) mx = &maps.x[1], mw = ws_of + 1, k0 = 0;  // the second pair of operands
         ok = umma::mbar_wait_warp(freed + 8 * s, phase);
         if (!ok) break;
         if (umma::elect_one()) {
-          if (rank == 0) tma::expect_tx(mine + 8 * s, 2 * S::kStageBytes);
+          if (rank == 0) tma::expect_tx(mine + 8 * s, 2 * (128 * 128 + wide * 128));
           const uint32_t bar = bars + 8 * s, xs = base + s * S::kStageBytes, ws = xs + 128 * 128;
           if constexpr (X_MN) {
             tma::load_2d_pair(xs, mx, m0, k0, bar);
@@ -187,7 +207,9 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           }
           if constexpr (W_MN) {
 #pragma unroll
-            for (int b = 0; b < BN / 128; ++b) tma::load_2d_pair(ws + b * 8192, mw, n0 + b * 64, k0, bar);
+            for (int b = 0; b < BN / 128; ++b) {
+              if (b * 64 < wide) tma::load_2d_pair(ws + b * 8192, mw, n0 + b * 64, k0, bar);
+            }
           } else {
             tma::load_2d_pair(ws, mw, k0, n0, bar);
           }
@@ -207,8 +229,9 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     const uint32_t filled = smem_addr(full), acc_freed = smem_addr(acc_empty);
     int s = 0, n = 0;
     uint32_t phase = 0;
-    for (int t = first; t < p.tiles && ok; t += step, ++n) {
+    for (int i = first; i < p.pieces && ok; i += step, ++n) {
       const int a = n & 1;
+      const uint32_t idesc = BN != 256 || i < p.whole ? p.idesc : p.idesc_half;
       ok = umma::mbar_wait_warp(acc_freed + 8 * a, ((n >> 1) & 1) ^ 1);
       umma::fence_after_sync();
       for (int kt = 0; kt < p.kt && ok; ++kt) {
@@ -220,7 +243,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
             umma::mma_pair<FP8>(tmem + a * BN, x0 + off + (X_MN ? ks * 128 : ks * 2), w0 + off + (W_MN ? ks * 128 : ks * 2),
-                                p.idesc, kt > 0 || ks > 0);
+                                idesc, kt > 0 || ks > 0);
           }
           umma::commit_pair(empty + s);
           if (kt == p.kt - 1) umma::commit_pair(acc_full + a);
@@ -241,22 +264,21 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     Staging stage{staging + (uint32_t)(warp - 4) * kStagingWarp};
     const bool half = p.half;
     int n = 0;
-    for (int t = first; t < p.tiles; t += step, ++n) {
+    for (int i = first; i < p.pieces; i += step, ++n) {
       const int a = n & 1;
-      const int g = t / p.tiles_mn;
-      int tm, tn;
-      locate(p, t - g * p.tiles_mn, tm, tn);
-      const int row0 = tm * 256 + (int)rank * 128 + w * 32, row = row0 + lane;
+      const Piece q = Piece::at<BN>(p, i);
+      const int row0 = q.tm * 256 + (int)rank * 128 + w * 32, row = row0 + lane;
       const bool live = row < p.rows;
       const uint32_t acc = tmem + a * BN + ((uint32_t)(32 * w) << 16);
-      constexpr int COLS = GATED ? BN / 2 : BN;
+      const int cols = (GATED ? BN / 2 : BN) / (q.whole ? 1 : 2);  // of y in this piece, from column col0 on
+      const int col0 = q.tn * (GATED ? BN / 2 : BN) + q.part * cols;
       Columns bias, scale0, scale1;
       auto read_columns = [&](int col) {
         if constexpr (!GATED) bias.read(p.bias, col, lane, p.features);
         if constexpr (FP8) scale0.read(p.w_scale[0], col, lane, p.features);
         if constexpr (FP8 && GATED) scale1.read(p.w_scale[1], col, lane, p.features);
       };
-      read_columns(tn * COLS + odd * 64);
+      read_columns(odd * 64 < cols ? col0 + odd * 64 : p.features);
       uint4 res[GATED ? 1 : 8];
       auto read_residual = [&](int col) {
         if constexpr (!GATED) {
@@ -265,7 +287,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           for (int j = 0; j < 8; ++j) res[j] = live && col + 8 * j < p.features ? *(r + j) : make_uint4(0, 0, 0, 0);
         }
       };
-      if (!GATED && p.residual) read_residual(tn * COLS + odd * 64);
+      if (!GATED && p.residual && odd * 64 < cols) read_residual(col0 + odd * 64);
       float xs = 1.f;
       if constexpr (FP8) xs = live ? *(p.x_scale + row) : 0.f;
       ok = umma::mbar_wait(acc_full + a, (n >> 1) & 1);
@@ -275,11 +297,11 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       }
       umma::fence_after_sync();
 #pragma unroll 1
-      for (int c = odd * 64; c < COLS; c += 128) {
-        const int col = tn * COLS + c;
+      for (int c = odd * 64; c < cols; c += 128) {
+        const int col = col0 + c;
         if (col >= p.features || row0 >= p.rows) break;
         const Columns b = bias, s0 = scale0, s1 = scale1;
-        read_columns(c + 128 < COLS ? col + 128 : p.features);
+        read_columns(c + 128 < cols ? col + 128 : p.features);
         uint32_t out[32];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -288,7 +310,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           umma::ld_32x32b_x32(v, acc + c + 32 * h);
           if constexpr (GATED) {
             float u[32];
-            umma::ld_32x32b_x32(u, acc + BN / 2 + c + 32 * h);
+            umma::ld_32x32b_x32(u, acc + cols + c + 32 * h);
             umma::wait_ld();
             if constexpr (FP8) {
 #pragma unroll
@@ -337,8 +359,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             for (int i = 0; i < 16; ++i) out[16 * h + i] = pack_out<is_half()>(v[2 * i], v[2 * i + 1]);
           });
         }
-        if (!GATED && p.residual && c + 128 < COLS) read_residual(col + 128);
-        stage.store64(out, lane, &maps.y[g], col, row0, p.features, p.rows);
+        if (!GATED && p.residual && c + 128 < cols) read_residual(col + 128);
+        stage.store64(out, lane, &maps.y[q.product], col, row0, p.features, p.rows);
       }
       umma::fence_before_sync();
       __syncwarp();
@@ -361,24 +383,30 @@ int launch(const Product& p, int device, int sms, cudaStream_t s) {
   Params q{};
   const int esz = FP8 ? 1 : 2, kb = FP8 ? 128 : 64;
   const int xr = X_MN ? 64 : 128, wr = W_MN ? 64 : BN / 2;
+  constexpr int COLS = GATED ? BN / 2 : BN;
+  q.rows = (int)p.rows, q.features = p.features;
+  q.tiles_n = (p.features + COLS - 1) / COLS;
+  q.tiles_mn = (int)((p.rows + 255) / 256) * q.tiles_n;
+  const int tiles = q.tiles_mn * (p.group ? 2 : 1), rest = tiles % (sms / 2);
+  const bool halves = BN == 256 && rest > 0 && 2 * rest <= sms / 2;
+  q.whole = halves ? tiles - rest : tiles;
+  q.pieces = halves ? tiles + rest : tiles;
   bool ok = true;
   for (int i = 0; i < 2 && ok; ++i) {  // (a second operand or output that is not there is not asked for either)
     ok = (!p.x[i] || (X_MN ? tma::encode_2d(&maps.x[i], p.x[i], esz, p.rows, p.depth, p.x_stride, xr)
                            : tma::encode_2d(&maps.x[i], p.x[i], esz, p.depth, p.rows, p.x_stride, xr))) &&
          (!p.w[i] || (W_MN ? tma::encode_2d(&maps.w[i], p.w[i], esz, p.features, p.depth, p.w_stride, wr)
                            : tma::encode_2d(&maps.w[i], p.w[i], esz, p.depth, p.features, p.w_stride, wr))) &&
+         (!p.w[i] || W_MN || !halves || tma::encode_2d(&maps.w_half[i], p.w[i], esz, p.depth, p.features, p.w_stride, BN / 4)) &&
          (!p.y[i] || tma::encode_2d(&maps.y[i], p.y[i], 2, p.features, p.rows, p.features, 32)) &&
          (!p.save[i] || tma::encode_2d(&maps.save[i], p.save[i], 4, p.features, p.rows, p.features, 32));
   }
   if (!ok) return JLA_ERR_CUDA;
-  constexpr int COLS = GATED ? BN / 2 : BN;
-  q.rows = (int)p.rows, q.features = p.features;
-  q.tiles_n = (p.features + COLS - 1) / COLS;
-  q.tiles_mn = (int)((p.rows + 255) / 256) * q.tiles_n;
-  q.tiles = q.tiles_mn * (p.group ? 2 : 1);
   q.kt0 = (p.depth + kb - 1) / kb;
   q.kt = q.kt0 * (p.pair ? 2 : 1);
   q.idesc = FP8 ? umma::instr_desc_e4m3(256, BN) : umma::instr_desc(256, BN, p.dtype == JLA_DTYPE_BF16, X_MN, W_MN);
+  q.idesc_half = FP8 ? umma::instr_desc_e4m3(256, BN / 2)
+                     : umma::instr_desc(256, BN / 2, p.dtype == JLA_DTYPE_BF16, X_MN, W_MN);
   q.act = p.act, q.half = p.out_dtype == JLA_DTYPE_F16, q.saves = p.save[0] != nullptr;
   q.x_scale = p.x_scale, q.w_scale[0] = p.w_scale[0], q.w_scale[1] = p.w_scale[1], q.bias = p.bias, q.residual = p.residual;
   q.status = tc_status_ptr();
@@ -389,7 +417,7 @@ int launch(const Product& p, int device, int sms, cudaStream_t s) {
   auto* kern = product_kernel<BN, X_MN, W_MN, FP8, GATED>;
   static std::atomic<uint64_t> allowed{0};
   JLA_CUDA_OK(allow_smem(kern, S::kSmem, device, allowed));
-  const int pairs = sms / 2 < q.tiles ? sms / 2 : q.tiles;
+  const int pairs = sms / 2 < q.pieces ? sms / 2 : q.pieces;
   ProfScope scope(kProfProduct, s);
   JLA_CUDA_OK(launch_overlapped(kern, dim3(2 * pairs), dim3(kThreads), S::kSmem, s, 0, maps, q));  // (the kernel has its cluster size)
   return JLA_OK;
@@ -402,7 +430,7 @@ bool narrow(const Product& p) { return p.features * (p.gated ? 2 : 1) <= 128; }
 template <bool X_MN, bool W_MN, bool FP8, bool GATED>
 int pick(const Product& p, int dev, int sms, cudaStream_t s) {
   return narrow(p) ? launch<128, X_MN, W_MN, FP8, GATED>(p, dev, sms, s)
-                        : launch<256, X_MN, W_MN, FP8, GATED>(p, dev, sms, s);
+                   : launch<256, X_MN, W_MN, FP8, GATED>(p, dev, sms, s);
 }
 
 }  // namespace

@@ -133,7 +133,8 @@ def test_linear_gradients(rows, depth, out, dtype, act, bias, residual):
 # Every kernel and tile width: few tokens (16, 32, 64 or 128 of them a block), pairs of CTAs (128 or 256 columns a tile, one
 # tile a pair and several).
 KERNELS = [(5, 2048, 136), (20, 520, 200), (50, 1000, 72), (100, 2048, 264), (100, 72, 2000), (1500, 4096, 24), (2100, 72, 56),
-           (8300, 72, 56), (8300, 264, 72), (8300, 136, 136), (5000, 72, 1000), (2100, 520, 1000), (18900, 72, 256)]
+           (8300, 72, 56), (8300, 264, 72), (8300, 136, 136), (5000, 72, 1000), (2100, 520, 1000), (8300, 72, 2600), (9400, 136, 264),
+           (18900, 72, 256)]
 
 
 @pytest.mark.parametrize("rows, depth, out", KERNELS)
@@ -214,7 +215,7 @@ def _e4m3(x):
 
 @pytest.mark.parametrize("rows, depth, out", [(1, 64, 64), (1, 16, 8), (5, 2048, 136), (33, 208, 1000), (100, 4096, 72),
                                               (200, 144, 264), (300, 16, 200), (1003, 1024, 520), (18900, 80, 256),
-                                              (20, 4096, 136), (60, 4096, 136), (8300, 80, 56), (8300, 80, 200), (5000, 144, 1000)])
+                                              (20, 4096, 136), (60, 4096, 136), (8300, 80, 56), (8300, 80, 200), (5000, 144, 1000), (9400, 80, 264)])
 @pytest.mark.parametrize("out_dtype", DTYPES)
 def test_e4m3(rows, depth, out, out_dtype):
     dtype = DTYPES[out_dtype]
