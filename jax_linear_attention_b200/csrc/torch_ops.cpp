@@ -387,13 +387,30 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
   }
 };
 
+// Widths that the kernels do not take as they are: zeros to the next multiple, in copies that autograd sees through.
+struct Padding {
+  int64_t out, more_in, more_out;
+  Padding(const Tensor& w) {
+    const int64_t step = w.scalar_type() == at::kFloat8_e4m3fn ? 16 : 8;
+    out = w.size(0), more_in = (step - w.size(1) % step) % step, more_out = (8 - out % 8) % 8;
+  }
+  bool needed() const { return more_in || more_out; }
+  static Tensor wider(const Tensor& t, int64_t cols, int64_t rows = 0) {
+    if (!t.defined() || (!cols && !rows)) return t;
+    const std::vector<int64_t> by = rows ? std::vector<int64_t>{0, cols, 0, rows} : std::vector<int64_t>{0, cols};
+    if (t.scalar_type() != at::kFloat8_e4m3fn) return at::constant_pad_nd(t, by, 0);
+    return at::constant_pad_nd(t.view(at::kByte), by, 0).view(at::kFloat8_e4m3fn);
+  }
+  Tensor cut(const Tensor& y) const { return more_out ? y.narrow(-1, 0, out).contiguous() : y; }
+};
+
 // The checks that both products share; `type` becomes the output's dtype.
 bool operands(const Tensor& x, const Tensor& w, const Tensor& x_scale, std::initializer_list<const Tensor*> scales,
               const py::handle& dtype_, at::ScalarType& type) {
   if (!x.defined() || !w.defined() || !x.is_cuda() || !on(w, x) || x.dim() < 1 || w.dim() != 2) return false;
   const at::ScalarType t = x.scalar_type();
-  const int64_t out = w.size(0), depth = w.size(1), step = t == at::kFloat8_e4m3fn ? 16 : 8;
-  if (w.scalar_type() != t || x.size(-1) != depth || depth < step || depth % step || out < 8 || out % 8) return false;
+  const int64_t out = w.size(0), depth = w.size(1);
+  if (w.scalar_type() != t || x.size(-1) != depth || depth < 1 || out < 1 || depth > (1 << 24) || out > (1 << 24)) return false;
   type = kNone;
   if (!take_dtype(dtype_, type)) return false;
   if (t != at::kFloat8_e4m3fn) {
@@ -432,10 +449,17 @@ py::object linear(const py::handle& x_, const py::handle& weight_, const py::han
   Tensor y;
   {
     py::gil_scoped_release unlocked;
-    w = aligned(w);
-    if (bias.defined()) bias = aligned(bias.scalar_type() == at::kFloat ? bias : bias.to(at::kFloat));
+    if (bias.defined() && bias.scalar_type() != at::kFloat) bias = bias.to(at::kFloat);
+    const Padding pad(w);
+    if (pad.needed()) {
+      x = pad.wider(x, pad.more_in), w = pad.wider(w, pad.more_in, pad.more_out), bias = pad.wider(bias, pad.more_out);
+      residual = pad.wider(residual, pad.more_out), w_scale = pad.wider(w_scale, pad.more_out);
+    }
+    w = aligned(w), bias = aligned(bias);
     y = grads ? Linear::apply(x, w, maybe(bias), maybe(residual), act)
-              : linear_fwd(rows_of(x, w.size(1)), w, aligned(x_scale), aligned(w_scale), bias, act, aligned(residual), shape, type, nullptr);
+              : linear_fwd(rows_of(x, w.size(1)), w, aligned(x_scale), aligned(w_scale), bias, act, aligned(residual),
+                           out_shape(x, w.size(0)), type, nullptr);
+    y = pad.cut(y);
   }
   return py::cast(y);
 }
@@ -454,10 +478,17 @@ py::object gated_linear(const py::handle& x_, const py::handle& gate_, const py:
   Tensor h;
   {
     py::gil_scoped_release unlocked;
+    const Padding pad(gate);
+    if (pad.needed()) {
+      x = pad.wider(x, pad.more_in);
+      gate = pad.wider(gate, pad.more_in, pad.more_out), up = pad.wider(up, pad.more_in, pad.more_out);
+      g_scale = pad.wider(g_scale, pad.more_out), u_scale = pad.wider(u_scale, pad.more_out);
+    }
     gate = aligned(gate), up = aligned(up);
     h = grads ? GatedLinear::apply(x, gate, up, act)
               : gated_fwd(rows_of(x, gate.size(1)), gate, up, aligned(x_scale), aligned(g_scale), aligned(u_scale), act,
                           out_shape(x, gate.size(0)), type, nullptr, nullptr);
+    h = pad.cut(h);
   }
   return py::cast(h);
 }

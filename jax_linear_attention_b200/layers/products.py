@@ -45,9 +45,8 @@ def _refuse(name: str, x, weights, scales, x_scale, out_dtype):
     if any(t.device != x.device for t in weights):
         raise ValueError(f"{name}: the weights must be on {x.device}")
     out, depth = w.shape
-    step = 16 if x.dtype == _E4M3 else 8
-    if depth < step or depth % step or out < 8 or out % 8:
-        raise ValueError(f"{name}: in features must be a multiple of {step} and out features of 8; got {depth} and {out}")
+    if not (1 <= depth <= 1 << 24 and 1 <= out <= 1 << 24):
+        raise ValueError(f"{name}: in and out features must be 1 .. 2^24; got {depth} and {out}")
     if x.dtype != _E4M3:
         if x_scale is not None or any(s is not None for s in scales):
             raise ValueError(f"{name}: scales go with e4m3 operands only")
@@ -66,11 +65,12 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
            out_dtype=None):
     """``act(x @ weight.T + bias) + residual``, in one launch.
 
-    ``x [..., in]`` and ``weight [out, in]`` in bf16 or f16 (``in`` and ``out`` multiples of 8), ``bias [out]``, ``residual
-    [..., out]`` in the output's dtype; ``activation`` is None, ``"silu"``, ``"gelu"`` (tanh form) or ``"sigmoid"``. The rows of
-    ``x`` may lie apart (a slice of a wider tensor). Gradients of ``x``, ``weight``, ``bias`` and ``residual``.
+    ``x [..., in]`` and ``weight [out, in]`` in bf16 or f16, ``bias [out]``, ``residual [..., out]`` in the output's dtype;
+    ``activation`` is None, ``"silu"``, ``"gelu"`` (tanh form) or ``"sigmoid"``. The rows of ``x`` may lie apart (a slice of a wider
+    tensor). Gradients of ``x``, ``weight``, ``bias`` and ``residual``. ``in`` and ``out`` that are no multiples of 8 (``in`` of 16
+    in e4m3) cost copies of the operands with zeros up to the next one: lay such weights out wider where that counts.
 
-    e4m3 operands (``in`` a multiple of 16) take ``x_scale [...]`` and ``weight_scale [out]`` in float32: the product is that
+    e4m3 operands take ``x_scale [...]`` and ``weight_scale [out]`` in float32: the product is that
     of ``x * x_scale[..., None]`` and ``weight * weight_scale[:, None]``; the output is bf16, or f16 with ``out_dtype``. This
     form has no gradient and is refused where one would be recorded.
     """
@@ -92,8 +92,7 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
 def gated_linear(x, w_gate, w_up, *, activation: str = "silu", x_scale=None, gate_scale=None, up_scale=None, out_dtype=None):
     """``act(x @ w_gate.T) * (x @ w_up.T)``, both products, the activation and their product in one launch.
 
-    ``x [..., in]``, ``w_gate`` and ``w_up [out, in]`` in bf16 or f16 (``in`` and ``out`` multiples of 8); ``activation`` is
-    ``"silu"``, ``"gelu"`` (tanh form) or ``"sigmoid"``. Gradients of ``x`` and both weights. e4m3 operands take ``x_scale
+    ``x [..., in]``, ``w_gate`` and ``w_up [out, in]`` in bf16 or f16 (widths as in ``linear``); ``activation`` is ``"silu"``, ``"gelu"`` (tanh form) or ``"sigmoid"``. Gradients of ``x`` and both weights. e4m3 operands take ``x_scale
     [...]``, ``gate_scale [out]`` and ``up_scale [out]`` as in ``linear``, without gradients.
     """
     act = _code("gated_linear", activation, ("silu", "gelu", "sigmoid"))

@@ -243,6 +243,62 @@ def test_kernels_that_overlap_see_what_was_written_before(rows):
         assert bool((a == c).all())
 
 
+def test_two_host_threads_at_once():
+    import threading
+
+    w = _weights(torch.bfloat16)
+    for t in w.values():
+        t.requires_grad_()
+    data = [[torch.randn(2, rows, D, device="cuda").bfloat16() for _ in range(2)] for rows in (40, 500)]
+    leaves = [w[n] for n in ("qkv", "gate", "up", "down", "n1")]
+
+    def step(x, s):
+        y, stream, _, _ = block(x, s, w)
+        return [y.detach(), *torch.autograd.grad(y, leaves, stream.detach())]
+
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(8):
+                    got[i] = step(*data[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as err:  # noqa: BLE001 (shown by the assertion below)
+            errors.append(err)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, b in zip(want, got):
+        # (the layers around these operators add gradients up with atomics: equal to a rounding, not to the bit)
+        assert bool((a[0] == b[0]).all()) and all(_rel(q, p) <= 2.0 ** -7 for p, q in zip(a[1:], b[1:]))
+
+
+def test_one_tensor_for_several_arguments():
+    x = torch.randn(64, 64, device="cuda").bfloat16().requires_grad_()
+    n, dy = torch.ones(64, device="cuda"), torch.randn(64, 64, device="cuda").bfloat16()
+    a, b = (x.detach().clone().requires_grad_() for _ in range(2))
+    for call in (lambda p, q: layers.linear(p, q), lambda p, q: layers.rms_norm(p, n, residual=q)[0]):
+        one, = torch.autograd.grad(call(x, x), [x], dy)
+        two = torch.autograd.grad(call(a, b), [a, b], dy)
+        assert bool((one == two[0] + two[1]).all())
+    c = x.detach().clone().requires_grad_()
+    for call in (lambda p, q, r: layers.linear(p, q, residual=r, activation="silu"), lambda p, q, r: layers.gated_linear(p, q, r)):
+        one, = torch.autograd.grad(call(x, x, x), [x], dy)
+        three = torch.autograd.grad(call(a, b, c), [a, b, c], dy)
+        # three terms, added two by two in whatever order: two roundings of half a step each, of sums no larger than all terms'
+        size = sum(t.double().abs() for t in three)
+        assert bool(((one.double() - sum(t.double() for t in three)).abs() <= 2 * 2.0 ** -8 * size).all())
+    y, stream = layers.rms_norm(x, n, residual=x)
+    assert bool((stream == 2 * x).all())
+
+
 def test_offsets_beyond_32_bits():
     rows, dim = 1_100_000, 2048  # 2.25e9 elements
     x = torch.randn(rows, dim, device="cuda", dtype=torch.bfloat16)

@@ -130,6 +130,18 @@ def test_linear_gradients(rows, depth, out, dtype, act, bias, residual):
     _check_linear_gradients(rows, depth, out, DTYPES[dtype], act, bias, residual)
 
 
+@pytest.mark.parametrize("rows, depth, out", [(1, 1, 1), (5, 7, 3), (30, 64, 6), (300, 100, 12), (130, 33, 257), (9000, 70, 50)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_any_width(rows, depth, out, dtype):
+    dtype = DTYPES[dtype]
+    t = _inputs(rows, depth, out, dtype, bias=True, residual=True, seed=9)
+    y = layers.linear(t["x"], t["w"], t["b"], activation="silu", residual=t["r"])
+    assert y.shape == (rows, out) and y.is_contiguous()
+    _check_linear(t, "silu", y, dtype)
+    _check_linear_gradients(rows, depth, out, dtype, "gelu", True, True)
+    _check_gated(rows, depth, out, dtype, "silu", True)
+
+
 # Every kernel and tile width: few tokens (16, 32, 64 or 128 of them a block), pairs of CTAs (128 or 256 columns a tile, one
 # tile a pair and several).
 KERNELS = [(5, 2048, 136), (20, 520, 200), (50, 1000, 72), (100, 2048, 264), (100, 72, 2000), (1500, 4096, 24), (2100, 72, 56),
@@ -215,7 +227,7 @@ def _e4m3(x):
 
 @pytest.mark.parametrize("rows, depth, out", [(1, 64, 64), (1, 16, 8), (5, 2048, 136), (33, 208, 1000), (100, 4096, 72),
                                               (200, 144, 264), (300, 16, 200), (1003, 1024, 520), (18900, 80, 256),
-                                              (20, 4096, 136), (60, 4096, 136), (8300, 80, 56), (8300, 80, 200), (5000, 144, 1000), (9400, 80, 264)])
+                                              (20, 4096, 136), (60, 4096, 136), (3, 7, 5), (300, 100, 12), (8300, 80, 56), (8300, 80, 200), (5000, 144, 1000), (9400, 80, 264)])
 @pytest.mark.parametrize("out_dtype", DTYPES)
 def test_e4m3(rows, depth, out, out_dtype):
     dtype = DTYPES[out_dtype]
@@ -374,6 +386,25 @@ def test_only_what_is_asked_for():
         assert bool((got == want).all())
 
 
+def test_one_dimension_and_other_biases():
+    t = _inputs(3, 64, 72, torch.bfloat16, bias=True, residual=True)
+    q, s = _e4m3(t["x"].float())
+    qw, sw = _e4m3(t["w"].float())
+    want = layers.linear(q, qw, x_scale=s, weight_scale=sw)
+    assert bool((layers.linear(q[1], qw, x_scale=s[1], weight_scale=sw) == want[1]).all())
+    b16 = t["b"].bfloat16().requires_grad_()  # a bias in 16 bits is used as it is, and so is its gradient's type
+    y = layers.linear(t["x"], t["w"], b16)
+    assert bool((y == layers.linear(t["x"], t["w"], b16.detach().float())).all())
+    g, = torch.autograd.grad(y, [b16], t["dy"])
+    assert g.dtype == torch.bfloat16
+    _close(g, t["dy"].double().sum(0), 2.0 ** -8 * t["dy"].double().sum(0).abs() + 1e-5)
+    r = t["r"].clone().requires_grad_()  # the residual alone
+    g, = torch.autograd.grad(layers.linear(t["x"], t["w"], t["b"], residual=r, activation="silu"), [r], t["dy"])
+    assert bool((g == t["dy"]).all())
+    g, = torch.autograd.grad(layers.linear(t["x"], t["w"], residual=r), [r], t["dy"])
+    assert bool((g == t["dy"]).all())
+
+
 def test_refusals():
     t = _inputs(4, 64, 72, torch.bfloat16, bias=True, residual=True, gated=True)
     x, w, up, b, r = (t[n] for n in ("x", "w", "up", "b", "r"))
@@ -381,8 +412,8 @@ def test_refusals():
     qw, sw = _e4m3(w.float())
     for call, text in (
             (lambda: layers.linear(x, w.half()), "share one of"), (lambda: layers.linear(x.float(), w.float()), "share one of"),
-            (lambda: layers.linear(x[:, :56], w), "expected x"), (lambda: layers.linear(x[:, :60], w[:, :60].contiguous()), "multiple"),
-            (lambda: layers.linear(x, w[:70]), "of 8"), (lambda: layers.linear(x, w, b[:64]), "bias"),
+            (lambda: layers.linear(x[:, :56], w), "expected x"), (lambda: layers.linear(x[:, :0], w[:, :0]), "features"),
+            (lambda: layers.linear(x, w[:0]), "features"), (lambda: layers.linear(x, w, b[:64]), "bias"),
             (lambda: layers.linear(x, w, b.cpu()), "bias"), (lambda: layers.linear(x, w, residual=r.float()), "residual"),
             (lambda: layers.linear(x, w, residual=r[:1]), "residual"), (lambda: layers.linear(x, w, x_scale=s), "scales"),
             (lambda: layers.linear(x, w, out_dtype=torch.float16), "out_dtype"), (lambda: layers.linear(q, qw), "x_scale"),

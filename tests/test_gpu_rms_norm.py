@@ -156,6 +156,9 @@ def test_shapes_strides_and_empty():
     assert bool((layers.rms_norm(wide[:, 3:99], w) == layers.rms_norm(x, w)).all())
     odd = torch.zeros(24 * 96 + 1, dtype=torch.float16, device="cuda")[1:].view(24, 96).copy_(x)  # not on 16 bytes
     assert bool((layers.rms_norm(odd, w) == layers.rms_norm(x, w)).all())
+    assert bool((layers.rms_norm(x[3], w) == layers.rms_norm(x, w)[3]).all())
+    q, s = layers.rms_norm(x[3], w, out_dtype=torch.float8_e4m3fn)
+    assert q.shape == (96,) and s.shape == ()
     assert layers.rms_norm(x[:0], w).shape == (0, 96)
     q, s, t = layers.rms_norm(x[:0], w, residual=r[:0], out_dtype=torch.float8_e4m3fn)
     assert q.shape == t.shape == (0, 96) and s.shape == (0,)
