@@ -8,9 +8,11 @@
 // The kernels are reached through the C ABI (include/jla_b200.h) of the library that the Python side has loaded: bind() gets
 // the addresses of its entry points. A call that these functions do not take comes back as None, and the Python side
 // says what is wrong with it.
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
@@ -132,6 +134,22 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// Called by a node's backward pass. While an eager graph of a leaf lives, autograd hands the leaf's gradient over on that graph's
+// stream. Where that is the default stream, which takes no part in a capture, the hand-over would break the capture.
+void refuse_broken_capture() {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& next = node->next_edge(i).function;
+    if (!next || !node->task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad*>(next.get())) continue;
+    const auto stream = next->stream();
+    TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
+                "an eager autograd graph of one of these leaves is alive on the default stream: drop its outputs before "
+                "the backward pass is captured");
+  }
+}
+
 // A tensor, None (undefined) or something else (false).
 bool take(const py::handle& h, Tensor& t) {
   if (h.is_none()) return true;
@@ -187,6 +205,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     return {n.y, n.stream};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_broken_capture();
     const bool again = at::GradMode::is_enabled();
     variable_list out;
     {
@@ -317,6 +336,7 @@ struct Linear : torch::autograd::Function<Linear> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_broken_capture();
     const bool again = at::GradMode::is_enabled();
     variable_list out;
     {
@@ -362,6 +382,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     return h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_broken_capture();
     const bool again = at::GradMode::is_enabled();
     variable_list out;
     {

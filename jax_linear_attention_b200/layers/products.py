@@ -13,6 +13,8 @@ do not see and float32 ones would.
 Forward is one launch, of a kernel for many tokens or of one for few (``csrc/product_tc.cu``, ``csrc/few_tokens.cu``).
 Backward, ``dx`` and ``dW`` are one launch each (both halves of a gated block together), after one for the activation's
 gradient and the bias's where there are any. Before an activation the product is kept in float32 for the backward pass.
+A backward pass is captured into a graph like any other work, but not while an eager autograd graph of its leaves is alive on the
+default stream: that raises.
 """
 
 from __future__ import annotations

@@ -189,6 +189,43 @@ def test_training_step_captured_and_replayed(rows):
             assert bool((a == c).all())
 
 
+@pytest.mark.parametrize("op", ["rms_norm", "linear", "gated_linear"])
+def test_capture_while_an_eager_graph_lives(op):
+    """The leaves' gradients would be handed over on the eager graph's stream, outside of the capture: refused, until that
+    graph is gone or where it is another leaf's."""
+    x, w = (torch.randn(64, 64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    n = torch.ones(64, device="cuda", requires_grad=True)
+    second = n if op == "rms_norm" else w
+    call = {"rms_norm": lambda: layers.rms_norm(x, n), "linear": lambda: layers.linear(x, w),
+            "gated_linear": lambda: layers.gated_linear(x, w, w)}[op]
+
+    def step(leaves):
+        y = call()
+        return torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+    want = step([x, second])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step([x, second])
+    torch.cuda.synchronize()
+    alive = call()
+    for leaves in ([x, second], [second]):
+        with pytest.raises(RuntimeError, match="eager autograd graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                step(leaves)
+    del alive
+    alive = second * 2 if op == "rms_norm" else second + 1  # of the second leaf only
+    for leaves, at in (([x], 0), ([x, second], None)):
+        if at is None:
+            del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(leaves)
+        graph.replay()
+        assert all(bool((a == b).all()) for a, b in zip(out, want))
+
+
 def test_two_streams_at_once():
     w = [_weights(torch.bfloat16, seed) for seed in range(2)]
     x = [torch.randn(2, 600, D, device="cuda").bfloat16() for _ in range(2)]
