@@ -134,6 +134,16 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// A saved tensor as a backward pass gets it. Saved-tensor hooks (offloading, compression) may hand back another tensor than
+// the one that was saved: its strides and its alignment count for nothing here, and what else differs is refused, since the
+// kernels would read outside of it or read it wrongly.
+Tensor restored(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+  TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided && t.sizes() == shape && t.scalar_type() == type &&
+                        t.device() == like.device(),
+                    "a saved tensor came back from its hook with another shape, dtype or device");
+  return t;
+}
+
 // Called by a node's backward pass. While an eager graph of a leaf lives, autograd hands the leaf's gradient over on that graph's
 // stream. Where that is the default stream, which takes no part in a capture, the hand-over would break the capture.
 void refuse_broken_capture() {
@@ -199,6 +209,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const Tensor residual = residual_.value_or(Tensor());
     Norm n = norm_fwd(x, residual, weight, eps, false, true);
     ctx->save_for_backward({x, residual, weight, n.rstd});
+    ctx->saved_data["residual"] = residual.defined();
     ctx->set_materialize_grads(false);
     if (!residual.defined()) return {n.y};
     if (!x.requires_grad() && !residual.requires_grad()) ctx->mark_non_differentiable({n.stream});  // the weight is not in it
@@ -211,14 +222,18 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     {
       at::AutoGradMode off(false);
       const variable_list saved = ctx->get_saved_variables();
-      const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2], &rstd = saved[3];
+      const bool has_residual = ctx->saved_data["residual"].toBool();
       Tensor dx, dw, dy = grads[0], ds = grads.size() > 1 ? grads[1] : Tensor();
       if (!dy.defined()) {
         dx = ds;  // only the stream was used
       } else {
-        c10::cuda::OptionalCUDAGuard guard(x.device());
+        c10::cuda::OptionalCUDAGuard guard(dy.device());
         dy = aligned(dy), ds = aligned(ds);
-        const int64_t dim = x.size(-1), rows = x.numel() / dim;
+        const int64_t dim = dy.size(-1), rows = dy.numel() / dim;
+        const Tensor x = aligned(restored(saved[0], dy.sizes(), dy.scalar_type(), dy));
+        const Tensor residual = has_residual ? aligned(restored(saved[1], dy.sizes(), dy.scalar_type(), dy)) : Tensor();
+        const Tensor weight = aligned(restored(saved[2], {dim}, at::kFloat, dy));
+        const Tensor rstd = aligned(restored(saved[3], {rows}, at::kFloat, dy));
         dx = make(x.sizes(), x.scalar_type(), x);
         Tensor scratch;
         size_t bytes = 0;
@@ -231,7 +246,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
                                ptr(ds), ptr(dx), fmut(dw), ptr(scratch), bytes, stream_of(x)),
               "jla_rms_norm_bwd");
       }
-      out = {dx, dw, residual.defined() ? dx : Tensor(), Tensor()};
+      out = {dx, dw, has_residual ? dx : Tensor(), Tensor()};
     }
     return again ? once(out) : out;
   }
@@ -331,7 +346,7 @@ struct Linear : torch::autograd::Function<Linear> {
     Tensor y = linear_fwd(rows, weight, {}, {}, bias, act, aligned(residual), out_shape(x, weight.size(0)), x.scalar_type(),
                           act != JLA_ACT_NONE ? &z : nullptr);
     ctx->save_for_backward({rows.t, weight, z});
-    ctx->saved_data["cfg"] = std::vector<int64_t>{act, rows.rows, rows.stride, bias.defined(), residual.defined()};
+    ctx->saved_data["cfg"] = std::vector<int64_t>{act, bias.defined(), residual.defined()};
     ctx->saved_data["shape"] = x.sizes().vec();
     return y;
   }
@@ -342,15 +357,17 @@ struct Linear : torch::autograd::Function<Linear> {
     {
       at::AutoGradMode off(false);
       const variable_list saved = ctx->get_saved_variables();
-      const Tensor &x = saved[0], &weight = saved[1], &z = saved[2];
       const std::vector<int64_t> cfg = ctx->saved_data["cfg"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
-      const int64_t act = cfg[0], rows = cfg[1];
-      const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = cfg[3] && ctx->needs_input_grad(2);
-      c10::cuda::OptionalCUDAGuard guard(weight.device());
+      const int64_t act = cfg[0];
+      const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = cfg[1] && ctx->needs_input_grad(2);
+      c10::cuda::OptionalCUDAGuard guard(grads[0].device());
       const Tensor dy = aligned(grads[0]);
+      const int64_t depth = shape.back(), n = dy.size(-1), rows = dy.numel() / n;
+      const Rows x = rows_of(restored(saved[0], shape, dy.scalar_type(), dy), depth);
+      const Tensor weight = aligned(restored(saved[1], {n, depth}, dy.scalar_type(), dy));
+      const Tensor z = act != JLA_ACT_NONE ? aligned(restored(saved[2], {rows, n}, at::kFloat, dy)) : Tensor();
       Tensor dz = dy, db, dx, dw;
       if (need_b || (z.defined() && (need_x || need_w))) {
-        const int64_t n = weight.size(0);
         if (z.defined()) dz = make({rows, n}, weight.scalar_type(), weight);
         Tensor scratch;
         size_t bytes = 0;
@@ -364,8 +381,8 @@ struct Linear : torch::autograd::Function<Linear> {
               "jla_activation_bwd");
       }
       if (need_x) dx = input_grad(shape, rows, dz, weight, {}, {});
-      if (need_w) weight_grads(weight, rows, x, cfg[2], dz, dw, {}, nullptr);
-      out = {dx, dw, db, cfg[4] && ctx->needs_input_grad(cfg[3] ? 3 : 2) ? grads[0] : Tensor(), Tensor()};
+      if (need_w) weight_grads(weight, rows, x.t, x.stride, dz, dw, {}, nullptr);
+      out = {dx, dw, db, cfg[2] && ctx->needs_input_grad(cfg[1] ? 3 : 2) ? grads[0] : Tensor(), Tensor()};
     }
     return again ? once(out) : out;
   }
@@ -377,7 +394,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     Tensor g, u;
     Tensor h = gated_fwd(rows, gate, up, {}, {}, {}, act, out_shape(x, gate.size(0)), x.scalar_type(), &g, &u);
     ctx->save_for_backward({rows.t, gate, up, g, u});
-    ctx->saved_data["cfg"] = std::vector<int64_t>{act, rows.rows, rows.stride};
+    ctx->saved_data["act"] = act;
     ctx->saved_data["shape"] = x.sizes().vec();
     return h;
   }
@@ -388,20 +405,25 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     {
       at::AutoGradMode off(false);
       const variable_list saved = ctx->get_saved_variables();
-      const Tensor &x = saved[0], &gate = saved[1], &up = saved[2], &g = saved[3], &u = saved[4];
-      const std::vector<int64_t> cfg = ctx->saved_data["cfg"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
-      const int64_t rows = cfg[1], n = gate.size(0);
-      c10::cuda::OptionalCUDAGuard guard(gate.device());
+      const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+      const int64_t act = ctx->saved_data["act"].toInt();
+      c10::cuda::OptionalCUDAGuard guard(grads[0].device());
       const Tensor dh = aligned(grads[0]);
+      const int64_t depth = shape.back(), n = dh.size(-1), rows = dh.numel() / n;
+      const Rows x = rows_of(restored(saved[0], shape, dh.scalar_type(), dh), depth);
+      const Tensor gate = aligned(restored(saved[1], {n, depth}, dh.scalar_type(), dh));
+      const Tensor up = aligned(restored(saved[2], {n, depth}, dh.scalar_type(), dh));
+      const Tensor g = aligned(restored(saved[3], {rows, n}, at::kFloat, dh));
+      const Tensor u = aligned(restored(saved[4], {rows, n}, at::kFloat, dh));
       const Tensor dg = make({rows, n}, gate.scalar_type(), gate), du = make({rows, n}, gate.scalar_type(), gate);
-      check(abi.gated_activation_bwd(code(gate.scalar_type()), rows, (int)n, (int)cfg[0], fptr(g), fptr(u), ptr(dh), ptr(dg), ptr(du),
+      check(abi.gated_activation_bwd(code(gate.scalar_type()), rows, (int)n, (int)act, fptr(g), fptr(u), ptr(dh), ptr(dg), ptr(du),
                                      stream_of(gate)),
             "jla_gated_activation_bwd");
       Tensor dx, d_gate, d_up;
       const bool need_g = ctx->needs_input_grad(1), need_u = ctx->needs_input_grad(2);
       if (ctx->needs_input_grad(0)) dx = input_grad(shape, rows, dg, gate, du, up);
-      if (need_g) weight_grads(gate, rows, x, cfg[2], dg, d_gate, need_u ? du : Tensor(), need_u ? &d_up : nullptr);
-      else if (need_u) weight_grads(up, rows, x, cfg[2], du, d_up, {}, nullptr);
+      if (need_g) weight_grads(gate, rows, x.t, x.stride, dg, d_gate, need_u ? du : Tensor(), need_u ? &d_up : nullptr);
+      else if (need_u) weight_grads(up, rows, x.t, x.stride, du, d_up, {}, nullptr);
       out = {dx, d_gate, d_up, Tensor()};
     }
     return again ? once(out) : out;
