@@ -5,7 +5,8 @@
 // features (rows of W) fill the 128 TMEM lanes, BN tokens are the accumulator's columns, so that few tokens waste
 // neither tensor-core rows nor shared memory. The contraction is cut into up to eight parts, one for each CTA of a
 // cluster; the cluster's CTAs share out the tokens among themselves, push each other their partial sums over distributed
-// shared memory, and add the parts up in the order of the parts, every time the same.
+// shared memory, and add the parts up in the order of the parts, every time the same. A CTA with more than kPartSteps steps of
+// its own sums those in runs of as many, one after the other in the same accumulator, and joins them in a second one.
 //
 // Measured on a B200, weights from HBM: one token, 2048 -> 8512 bf16 8.2 us (35 MB; 5.3 at HBM's rate); 33 tokens, 4096 -> 2048 e4m3
 // 6.5 us; gated, four tokens, 2048 -> 5632 bf16 8.8 us warm, 13 us from HBM (46 MB). Of that about 0.8 us are set-up, 1.5 to 2.5 us
@@ -59,7 +60,8 @@ template <int BN, bool GATED> struct Shape {
   static constexpr int kSmem = kRing + kPartBytes + 1024;
   // TMEM columns: a load takes 32 from the start of an accumulator, also where the accumulator has 16
   static constexpr int kNeed = (GATED ? BN : 0) + (BN < 32 ? 32 : BN);
-  static constexpr int kCols = kNeed <= 32 ? 32 : kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : 256;
+  static_assert(kNeed <= 128, "twice as many where a CTA sums several runs of steps");
+  static constexpr int kCols = kNeed <= 32 ? 32 : kNeed <= 64 ? 64 : 128;
 };
 
 struct Quad {
@@ -98,13 +100,14 @@ __device__ __forceinline__ void finish(const Params& p, int token, int f, Quad v
   });
 }
 
-template <int BN, bool W_MN, bool FP8, bool GATED>
+// RUNS: some CTA has more than kPartSteps steps. (A kernel of its own: the tests for it cost one token, 2048 -> 8512, 0.6 us of 9.4.)
+template <int BN, bool W_MN, bool FP8, bool GATED, bool RUNS>
 __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_tokens_kernel(const __grid_constant__ Maps maps,
                                                                  const __grid_constant__ Params p, int split) {
   using S = Shape<BN, GATED>;
   constexpr int ST = S::kStages, NW = GATED ? 2 : 1;
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ __align__(8) uint64_t full[ST], empty[ST], done, drain, arrived;
+  __shared__ __align__(8) uint64_t full[ST], empty[ST], done, freed, drain, arrived;
   __shared__ uint32_t tmem_slot;
   const uint32_t base = (smem_addr(smem_dyn) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -135,6 +138,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_token
     tma::load_2d(xs, &maps.x[second ? 1 : 0], k0, m0, bar);
   };
   const int steps = k_hi - k_lo;
+  constexpr uint32_t kCols = RUNS ? 2 * S::kCols : S::kCols;
   int asked = steps < ST ? steps : ST;
   if (warp == 4) {
     if (umma::elect_one()) {
@@ -143,6 +147,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_token
         umma::mbar_init(empty + i, 1);
       }
       umma::mbar_init(&done, 1);
+      if constexpr (RUNS) umma::mbar_init(&freed, 4);
       umma::mbar_init(&drain, 1);
       umma::mbar_init(&arrived, 1);
       umma::mbar_init_fence();
@@ -151,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_token
     }
     __syncwarp();
   }
-  if (warp == 5) umma::tmem_alloc(&tmem_slot, S::kCols);
+  if (warp == 5) umma::tmem_alloc(&tmem_slot, kCols);
   umma::fence_before_sync();
   umma::cluster_arrive();  // (waited for before the first partial sums leave for another CTA)
   if (warp == 4) {  // the first copies wait for nobody
@@ -190,6 +195,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_token
     int s = 0;
     uint32_t phase = 0;
     for (int it = 0; it < steps; ++it) {
+      const int in_run = RUNS ? it % kPartSteps : it;
+      if (RUNS && in_run == 0 && it > 0) {  // the run before has been taken over
+        ok = umma::mbar_wait_warp(smem_addr(&freed), (it / kPartSteps - 1) & 1);
+        if (!ok) break;
+      }
       ok = umma::mbar_wait_warp(smem_addr(full) + 8 * s, phase);
       if (!ok) break;
       umma::fence_after_sync();
@@ -200,11 +210,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_token
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
             umma::mma_any<FP8>(tmem + i * BN, w0 + off + i * (S::kWeightBytes >> 4) + (W_MN ? ks * 128 : ks * 2),
-                               x0 + off + ks * 2, p.idesc, it > 0 || ks > 0);
+                               x0 + off + ks * 2, p.idesc, in_run > 0 || ks > 0);
           }
         }
         umma::commit(empty + s);
-        if (it == steps - 1) umma::commit(&done);
+        if ((RUNS && in_run == kPartSteps - 1) || it == steps - 1) umma::commit(&done);
       }
       __syncwarp();
       if (++s == ST) s = 0, phase ^= 1;
@@ -222,19 +232,35 @@ __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_token
     if constexpr (FP8 && GATED) ws1 = quad(p.w_scale[1] + f4);
     if (!GATED && p.bias) bias = quad(p.bias + f4);
   }
+  const uint32_t sums = tmem + (RUNS ? S::kCols : 0) + ((uint32_t)(32 * (warp & 3)) << 16);
   if (warp < 4) {
     ok = umma::mbar_wait(&done, 0);
     umma::fence_after_sync();
   }
+  if (RUNS && warp < 4) {
+    for (int it = 0, run = 0; it < steps; it += kPartSteps, ++run) {
+      if (run > 0) ok = umma::mbar_wait(&done, run & 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      umma::fence_after_sync();
+#pragma unroll 1
+      for (int c = 0; c < NW * BN; c += 16) umma::join_x16(sums + c, sums - S::kCols + c, run == 0);
+      umma::wait_st();
+      umma::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) umma::arrive_cluster(smem_addr(&freed));
+    }
+  }
   // This part's sums, [weight][token][128 features], over the ring, which is idle now. Column c of the accumulator is a token.
   if (warp < 4 && __all_sync(0xffffffffu, ok)) {
-    const uint32_t acc = tmem + ((uint32_t)(32 * warp) << 16);
     constexpr int CH = BN < 32 ? BN : 32;  // (of a load of 32 columns where there are 16, the last 16 are not looked at)
 #pragma unroll 1
     for (int c = 0; c < tokens; c += CH) {
       float v[NW][32];
 #pragma unroll
-      for (int i = 0; i < NW; ++i) umma::ld_32x32b_x32(v[i], acc + i * BN + c);
+      for (int i = 0; i < NW; ++i) umma::ld_32x32b_x32(v[i], sums + i * BN + c);
       umma::wait_ld();
 #pragma unroll
       for (int i = 0; i < NW; ++i) {
@@ -319,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<BN, GATED>::kCtas)) few_token
   umma::fence_before_sync();
   if (split > 1) umma::cluster_sync();  // the others' copies of this CTA's sums have arrived
   else __syncthreads();
-  if (warp == 5) umma::tmem_dealloc(tmem, S::kCols);
+  if (warp == 5) umma::tmem_dealloc(tmem, kCols);
 }
 
 template <int BN, bool W_MN, bool FP8, bool GATED>
@@ -348,8 +374,8 @@ int launch(const Product& p, int device, cudaStream_t s) {
     return JLA_ERR_CUDA;
   }
   const int tiles_f = (p.features + 127) / 128, tiles_m = (int)((p.rows + BN - 1) / BN);
-  auto* kern = few_tokens_kernel<BN, W_MN, FP8, GATED>;
-  static std::atomic<uint64_t> allowed{0};
+  auto* kern = few_tokens_kernel<BN, W_MN, FP8, GATED, false>;
+  static std::atomic<uint64_t> allowed{0}, allowed_runs{0};
   JLA_CUDA_OK(allow_smem(kern, S::kSmem, device, allowed));
   // Parts of the contraction: as many as there is room for at one time, each of at least two steps. (A cluster lies within
   // one of the GPU's groups of SMs, so fewer large clusters fit than their CTAs' number says; one that had to wait for
@@ -373,6 +399,10 @@ int launch(const Product& p, int device, cudaStream_t s) {
       split = c;
       break;
     }
+  }
+  if ((q.kt + split - 1) / split > kPartSteps) {
+    kern = few_tokens_kernel<BN, W_MN, FP8, GATED, true>;
+    JLA_CUDA_OK(allow_smem(kern, S::kSmem, device, allowed_runs));
   }
   ProfScope scope(kProfFewTokens, s);
   JLA_CUDA_OK(launch_overlapped(kern, dim3(tiles_f * split, tiles_m), dim3(kThreads), S::kSmem, s, split, maps, q, split));

@@ -72,6 +72,14 @@ __device__ __forceinline__ float2 unpack_out(uint32_t x) {
   else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
 }
 
+// Steps of the contraction (128 bytes of a row each: four instructions) that are summed in one accumulator. An instruction cuts
+// the sum off to float32's 24 bits where an addition would round it: up to 2^-23 of the sum each time, always to the same
+// side. 1024 of them are off by 2^-13 at most, a quarter of half a step of float16 (measured: 2e-5 of the result with random signs,
+// 6.5e-5 where all terms are positive; twice as many: 4e-5 and 1.5e-4, so that the gradient of a weight over 400k tokens would be off
+// by more than half a step). Longer contractions are summed in parts, and the parts joined with rounding. It also bounds what a
+// wait for a finished accumulator waits for: 256 steps are about 75 us, its limit is kSpinLimit polls, over 40 ms.
+constexpr int kPartSteps = 256;
+
 // One product (host view). "tokens" are the rows of y, "features" its columns; the contraction runs over `depth`, and over
 // the second pair of operands after the first where there is one (dx = dg Wg + du Wu).
 struct Product {

@@ -9,7 +9,8 @@
 // weight where gated): a warp fetches operand tiles of 128 bytes of contraction by TMA into a ring of 6 or 8 stages, one
 // thread of the leading CTA issues the products, eight warps of each CTA take finished accumulators out of TMEM (32 rows a
 // warp, a row a thread) through shared memory and TMA stores. Two sets of accumulators: the epilogue of one tile
-// runs under the products of the next. A pair reads an operand byte from L2 half as often as two CTAs of 128 x BN would.
+// runs under the products of the next. (Contractions of more than kPartSteps steps are summed in parts: one set is the running
+// part's, the other holds the sum of the parts.) A pair reads an operand byte from L2 half as often as two CTAs of 128 x BN would.
 // Tiles of a last round that would leave more than half of the pairs idle are taken in halves (1003 x 2048 x 6144 f16, 96
 // tiles on 74 pairs: 31 -> 27 us with silu; 700 x 2048 x 2048, 24 tiles: 19.5 -> 15.7 us).
 //
@@ -45,6 +46,7 @@ struct Params {
   int tiles_n, tiles_mn;        // tiles in a row of tiles, in one product
   int whole, pieces;            // tiles taken whole, and pieces in all: those and the halves of the others
   int kt0, kt;                  // steps of the contraction with the first pair of operands, and in all
+  int part;                     // steps that are summed in one accumulator (kt where they are few enough)
   uint32_t idesc, idesc_half;
   int act, half, saves;
   const float *x_scale, *w_scale[2], *bias;
@@ -227,14 +229,15 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     const uint64_t x0 = umma::smem_desc(base, X_MN ? 8192 : 16, 1024);
     const uint64_t w0 = umma::smem_desc(base + 128 * 128, W_MN ? 8192 : 16, 1024);
     const uint32_t filled = smem_addr(full), acc_freed = smem_addr(acc_empty);
+    const bool parts = p.part < p.kt;
     int s = 0, n = 0;
     uint32_t phase = 0;
-    for (int i = first; i < p.pieces && ok; i += step, ++n) {
-      const int a = n & 1;
+    for (int i = first, k0 = 0; i < p.pieces && ok; ++n) {  // (a piece, or one part of its contraction)
+      const int a = parts ? 0 : n & 1, k1 = k0 + p.part < p.kt ? k0 + p.part : p.kt;
       const uint32_t idesc = BN != 256 || i < p.whole ? p.idesc : p.idesc_half;
-      ok = umma::mbar_wait_warp(acc_freed + 8 * a, ((n >> 1) & 1) ^ 1);
+      ok = umma::mbar_wait_warp(acc_freed + 8 * a, ((parts ? n : n >> 1) & 1) ^ 1);
       umma::fence_after_sync();
-      for (int kt = 0; kt < p.kt && ok; ++kt) {
+      for (int kt = k0; kt < k1 && ok; ++kt) {
         ok = umma::mbar_wait_warp(filled + 8 * s, phase);
         if (!ok) break;
         umma::fence_after_sync();
@@ -243,14 +246,16 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
             umma::mma_pair<FP8>(tmem + a * BN, x0 + off + (X_MN ? ks * 128 : ks * 2), w0 + off + (W_MN ? ks * 128 : ks * 2),
-                                idesc, kt > 0 || ks > 0);
+                                idesc, kt > k0 || ks > 0);
           }
           umma::commit_pair(empty + s);
-          if (kt == p.kt - 1) umma::commit_pair(acc_full + a);
+          if (kt == k1 - 1) umma::commit_pair(acc_full + a);
         }
         __syncwarp();
         if (++s == ST) s = 0, phase ^= 1;
       }
+      k0 = k1;
+      if (k1 == p.kt) k0 = 0, i += step;
     }
     if (!ok) {  // products in flight read both CTAs' shared memory: wait for them
       if (umma::elect_one()) umma::commit_pair(&drain);
@@ -263,15 +268,47 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     const int w = warp & 3, odd = warp >= 8;
     Staging stage{staging + (uint32_t)(warp - 4) * kStagingWarp};
     const bool half = p.half;
+    auto release_accumulator = [&](int a) {
+      umma::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) umma::arrive_cluster(umma::map_rank(smem_addr(acc_empty + a), 0));
+    };
+    // A long contraction: its parts come one after the other in the first accumulator, their sum is kept in the second, each
+    // column by the warp that needs it in the end. (The products stand still while a part is taken over, which does not show: dW of 65536 x 2048 x 2048 345 us
+    // with and without.)
+    int joined = 0;
+    auto join = [&](int cols, uint32_t sum) {
+      for (int k0 = 0; k0 < p.kt; k0 += p.part, ++joined) {
+        const bool here = umma::mbar_wait(acc_full, joined & 1);
+        if (!__all_sync(0xffffffffu, here)) return false;
+        umma::fence_after_sync();
+#pragma unroll 1
+        for (int c = odd * 64; c < cols; c += 128) {
+#pragma unroll 1
+          for (int h = 0; h < (GATED ? 8 : 4); ++h) {
+            const uint32_t at = sum + c + 16 * (h & 3) + (h > 3 ? cols : 0);
+            umma::join_x16(at, at - BN, k0 == 0);
+          }
+        }
+        umma::wait_st();
+        release_accumulator(0);
+      }
+      return true;
+    };
+    const bool parts = p.part < p.kt;
     int n = 0;
     for (int i = first; i < p.pieces; i += step, ++n) {
-      const int a = n & 1;
+      const int a = parts ? 1 : n & 1;
       const Piece q = Piece::at<BN>(p, i);
       const int row0 = q.tm * 256 + (int)rank * 128 + w * 32, row = row0 + lane;
       const bool live = row < p.rows;
       const uint32_t acc = tmem + a * BN + ((uint32_t)(32 * w) << 16);
       const int cols = (GATED ? BN / 2 : BN) / (q.whole ? 1 : 2);  // of y in this piece, from column col0 on
       const int col0 = q.tn * (GATED ? BN / 2 : BN) + q.part * cols;
+      if (parts && !join(cols, acc)) {
+        ok = false;
+        break;
+      }
       Columns bias, scale0, scale1;
       auto read_columns = [&](int col) {
         if constexpr (!GATED) bias.read(p.bias, col, lane, p.features);
@@ -290,7 +327,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       if (!GATED && p.residual && odd * 64 < cols) read_residual(col0 + odd * 64);
       float xs = 1.f;
       if constexpr (FP8) xs = live ? *(p.x_scale + row) : 0.f;
-      ok = umma::mbar_wait(acc_full + a, (n >> 1) & 1);
+      if (!parts) ok = umma::mbar_wait(acc_full + a, (n >> 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
@@ -362,9 +399,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         if (!GATED && p.residual && c + 128 < cols) read_residual(col + 128);
         stage.store64(out, lane, &maps.y[q.product], col, row0, p.features, p.rows);
       }
-      umma::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) umma::arrive_cluster(umma::map_rank(smem_addr(acc_empty + a), 0));
+      if (!parts) release_accumulator(a);
     }
     if (lane == 0) tma::store_wait<0>();
   }
@@ -404,6 +439,8 @@ int launch(const Product& p, int device, int sms, cudaStream_t s) {
   if (!ok) return JLA_ERR_CUDA;
   q.kt0 = (p.depth + kb - 1) / kb;
   q.kt = q.kt0 * (p.pair ? 2 : 1);
+  const int parts = (q.kt + kPartSteps - 1) / kPartSteps;
+  q.part = (q.kt + parts - 1) / parts;  // (equal ones, but for the last)
   q.idesc = FP8 ? umma::instr_desc_e4m3(256, BN) : umma::instr_desc(256, BN, p.dtype == JLA_DTYPE_BF16, X_MN, W_MN);
   q.idesc_half = FP8 ? umma::instr_desc_e4m3(256, BN / 2)
                      : umma::instr_desc(256, BN / 2, p.dtype == JLA_DTYPE_BF16, X_MN, W_MN);

@@ -96,6 +96,27 @@ __device__ __forceinline__ void mma_any(uint32_t d_tmem, uint64_t a_desc, uint64
   }
 }
 
+// ---- sums in TMEM ------------------------------------------------------------------------------------------------
+// 16 columns of the 32 lanes of a warp: sum = part, or sum += part.
+__device__ __forceinline__ void ld_32x32b_x16(uint32_t (&r)[16], uint32_t taddr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void join_x16(uint32_t sum, uint32_t part, bool first) {
+  uint32_t v[16], t[16];
+  ld_32x32b_x16(v, part);
+  if (!first) ld_32x32b_x16(t, sum);
+  wait_ld();
+  if (!first) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(t[j]));
+  }
+  st_32x32b_x16(sum, v);
+}
+
 // ---- a pair of CTAs -----------------------------------------------------------------------------------------------
 // One warp of EACH CTA allocates (and at the end frees) the same number of columns.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t cols) {

@@ -7,8 +7,10 @@ A whole block is ``rms_norm`` -> ``linear`` -> the mixer -> ``linear`` with the 
 ``gated_linear`` -> ``linear`` with the residual. Operands are bf16 or f16 (with gradients), or e4m3 with one float32 scale a
 row of ``x`` and a row of the weight (serving; ``rms_norm`` leaves its output in that form). Products are summed in float32
 by the tensor cores, and everything up to the rounding of the result is float32. float32 operands are not taken: the tensor
-cores cut their sums off instead of rounding them (4e-6 of the result at a depth of 4096, 2e-5 at 16384), which 16-bit results
-do not see and float32 ones would.
+cores cut their sums off instead of rounding them (4e-6 of the result at a depth of 4096, 2e-5 at 16384 with random signs, 6.5e-5
+where all terms are positive), which 16-bit results do not see and float32 ones would. Contractions of more than 16384 (e4m3:
+32768) are summed in parts of that length, joined in float32 with rounding, so that this does not grow with the number of tokens
+that the gradient of a weight sums over.
 
 Forward is one launch, of a kernel for many tokens or of one for few (``csrc/product_tc.cu``, ``csrc/few_tokens.cu``).
 Backward, ``dx`` and ``dW`` are one launch each (both halves of a gated block together), after one for the activation's
