@@ -17,6 +17,8 @@
 #include <torch/extension.h>
 
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/jla_b200.h"
 
@@ -144,19 +146,28 @@ Tensor restored(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, con
   return t;
 }
 
-// Called by a node's backward pass. While an eager graph of a leaf lives, autograd hands the leaf's gradient over on that graph's
-// stream. Where that is the default stream, which takes no part in a capture, the hand-over would break the capture.
+// Called by a node's backward pass. Autograd hands a gradient over on the stream of the node that takes it. Where that is the
+// default stream, which takes no part in a capture, the hand-over breaks the capture: a leaf's node, while an eager graph of the
+// leaf lives, or a node of this graph that was made before the capture. So all nodes are looked at that this one's gradients go
+// to, directly or by way of others (a cast of a bias, a transposed or padded weight). Only a captured pass pays for it.
 void refuse_broken_capture() {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
-  for (size_t i = 0; i < node->num_outputs(); ++i) {
-    const auto& next = node->next_edge(i).function;
-    if (!next || !node->task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad*>(next.get())) continue;
-    const auto stream = next->stream();
-    TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
-                "an eager autograd graph of one of these leaves is alive on the default stream: drop its outputs before "
-                "the backward pass is captured");
+  std::vector<torch::autograd::Node*> open{node.get()};
+  std::unordered_set<torch::autograd::Node*> seen{node.get()};
+  while (!open.empty()) {
+    torch::autograd::Node* from = open.back();
+    open.pop_back();
+    for (size_t i = 0; i < from->num_outputs(); ++i) {
+      torch::autograd::Node* next = from->next_edge(i).function.get();
+      if (!next || !from->task_should_compute_output(i) || !seen.insert(next).second) continue;
+      const auto stream = next->stream();
+      TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
+                  "an eager autograd graph of one of these leaves is alive on the default stream, or a part of this graph was made "
+                  "there: drop its outputs before the backward pass is captured, and make the whole graph in the capture");
+      open.push_back(next);
+    }
   }
 }
 

@@ -16,7 +16,7 @@ Forward is one launch, of a kernel for many tokens or of one for few (``csrc/pro
 Backward, ``dx`` and ``dW`` are one launch each (both halves of a gated block together), after one for the activation's
 gradient and the bias's where there are any. Before an activation the product is kept in float32 for the backward pass.
 A backward pass is captured into a graph like any other work, but not while an eager autograd graph of its leaves is alive on the
-default stream: that raises.
+default stream, nor where a part of its graph was made there (a weight that was transposed before the capture): that raises.
 """
 
 from __future__ import annotations
