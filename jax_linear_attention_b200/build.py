@@ -4,7 +4,8 @@
 
 Every ``csrc/*.cu`` is compiled to an object (in parallel, only when its sources are newer than the
 object) and linked into ``jax_linear_attention_b200/libjla_b200.so``; ``csrc/torch_ops.cpp`` (the torch side of the layers
-whose host time matters most) becomes ``_torch_ops.so`` next to it. No GPU is needed to build.
+whose host time matters most) becomes ``_torch_ops.so`` next to it, for the torch and the Python that run the build (without
+torch, the library is all that is built). No GPU is needed to build.
 """
 
 from __future__ import annotations
@@ -12,6 +13,8 @@ from __future__ import annotations
 import argparse
 import concurrent.futures
 import glob
+import importlib.util
+import json
 import os
 import shutil
 import subprocess
@@ -56,7 +59,7 @@ def _compile(src: str, obj: str, verbose: bool) -> str:
     return obj
 
 
-def _build_torch_ops(verbose: bool) -> str:
+def _torch_ops_command() -> list[str]:
     import sysconfig
 
     import torch
@@ -64,20 +67,39 @@ def _build_torch_ops(verbose: bool) -> str:
 
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
     includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], cuda]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_ops",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f for path in includes for f in ("-isystem", path)), os.path.join(CSRC, "torch_ops.cpp"), "-o", TORCH_OPS,
-           *(f"-L{path}" for path in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
-           "-ltorch_python"]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_ops",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f for path in includes for f in ("-isystem", path)), os.path.join(CSRC, "torch_ops.cpp"), "-o", TORCH_OPS,
+            *(f"-L{path}" for path in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+            "-ltorch_python"]
+
+
+def _build_torch_ops(force: bool, verbose: bool) -> None:
+    """Makes ``_torch_ops.so`` where its sources are newer, or where it was made for another torch or Python or by another command
+    (which its file's time does not tell: ``_torch_ops.json`` beside the objects does)."""
+    import torch
+
+    cmd = _torch_ops_command()
+    made_by, note = dict(torch=torch.__version__, python=sys.version, command=cmd), os.path.join(OBJ, "_torch_ops.json")
+    try:
+        with open(note) as f:
+            same = json.load(f) == made_by
+    except (OSError, ValueError):
+        same = False
+    if same and not force and not _newer(TORCH_OPS, [cmd[cmd.index("-o") - 1], os.path.join(HERE, "..", "include", "jla_b200.h")]):
+        return
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"the torch side of the layers failed to build:\n{(proc.stdout + proc.stderr)[-6000:]}")
+    with open(note, "w") as f:
+        json.dump(made_by, f)
     if verbose:
         print(proc.stdout + proc.stderr)
-    return TORCH_OPS
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """Makes what is out of date; returns the library's path. Where the torch side fails, the library is there all the same; a
+    host without torch gets the library alone."""
     os.makedirs(OBJ, exist_ok=True)
     sources = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     headers = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(HERE, "..", "include", "*.h"))
@@ -92,16 +114,19 @@ def build(force: bool = False, verbose: bool = False) -> str:
     for path in stale:
         os.remove(path)
     with concurrent.futures.ThreadPoolExecutor(max_workers=8) as pool:
-        side = [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(HERE, "..", "include", "jla_b200.h")]
-        glue = pool.submit(_build_torch_ops, verbose) if force or _newer(TORCH_OPS, side) else None
+        glue = None
+        if importlib.util.find_spec("torch") is not None:
+            glue = pool.submit(_build_torch_ops, force, verbose)
         list(pool.map(lambda j: _compile(j[0], j[1], verbose), jobs))
-        if glue is not None:
-            glue.result()
     if jobs or stale or force or _newer(LIB, objs):
         cmd = [nvcc(), "-shared", "-o", LIB, *objs, "-lcudart"]
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError("link failed:\n" + proc.stdout + proc.stderr)
+    if glue is None:
+        print("no torch on this host: the library alone was built, without the torch side of the layers", file=sys.stderr)
+    else:
+        glue.result()
     return LIB
 
 
