@@ -338,13 +338,13 @@ Tensor input_grad(at::IntArrayRef shape, int64_t rows, const Tensor& dz, const T
   return dx;
 }
 
-// dw of dz, and dw2 of dz2 in the same launch where there is one
-void weight_grads(const Tensor& w, int64_t rows, const Tensor& x, int64_t stride, const Tensor& dz, Tensor& dw, const Tensor& dz2,
-                  Tensor* dw2) {
-  dw = make(w.sizes(), w.scalar_type(), w);
-  if (dw2) *dw2 = make(w.sizes(), w.scalar_type(), w);
-  check(abi.linear_bwd_weight(code(w.scalar_type()), rows, (int)w.size(1), (int)w.size(0), ptr(dz), ptr(dz2), ptr(x), stride, ptr(dw),
-                              dw2 ? ptr(*dw2) : nullptr, stream_of(w)),
+// dw [out, in] of dz, and dw2 of dz2 in the same launch where there is one
+void weight_grads(const Rows& x, const Tensor& dz, int64_t out, Tensor& dw, const Tensor& dz2, Tensor* dw2) {
+  const int64_t in = x.t.size(-1);
+  dw = make({out, in}, dz.scalar_type(), dz);
+  if (dw2) *dw2 = make({out, in}, dz.scalar_type(), dz);
+  check(abi.linear_bwd_weight(code(dz.scalar_type()), x.rows, (int)in, (int)out, ptr(dz), ptr(dz2), ptr(x.t), x.stride, ptr(dw),
+                              dw2 ? ptr(*dw2) : nullptr, stream_of(dz)),
         "jla_linear_bwd_weight");
 }
 
@@ -353,10 +353,12 @@ struct Linear : torch::autograd::Function<Linear> {
                         const std::optional<Tensor>& residual_, int64_t act) {
     const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
     const Rows rows = rows_of(x, weight.size(1));
+    const bool keep_z = act != JLA_ACT_NONE && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()));
     Tensor z;
     Tensor y = linear_fwd(rows, weight, {}, {}, bias, act, aligned(residual), out_shape(x, weight.size(0)), x.scalar_type(),
-                          act != JLA_ACT_NONE ? &z : nullptr);
-    ctx->save_for_backward({rows.t, weight, z});
+                          keep_z ? &z : nullptr);
+    // what the gradients that are wanted read, and nothing else: a frozen weight keeps no x alive
+    ctx->save_for_backward({weight.requires_grad() ? rows.t : Tensor(), x.requires_grad() ? weight : Tensor(), z});
     ctx->saved_data["cfg"] = std::vector<int64_t>{act, bias.defined(), residual.defined()};
     ctx->saved_data["shape"] = x.sizes().vec();
     return y;
@@ -374,25 +376,23 @@ struct Linear : torch::autograd::Function<Linear> {
       c10::cuda::OptionalCUDAGuard guard(grads[0].device());
       const Tensor dy = aligned(grads[0]);
       const int64_t depth = shape.back(), n = dy.size(-1), rows = dy.numel() / n;
-      const Rows x = rows_of(restored(saved[0], shape, dy.scalar_type(), dy), depth);
-      const Tensor weight = aligned(restored(saved[1], {n, depth}, dy.scalar_type(), dy));
-      const Tensor z = act != JLA_ACT_NONE ? aligned(restored(saved[2], {rows, n}, at::kFloat, dy)) : Tensor();
-      Tensor dz = dy, db, dx, dw;
-      if (need_b || (z.defined() && (need_x || need_w))) {
-        if (z.defined()) dz = make({rows, n}, weight.scalar_type(), weight);
+      Tensor z, dz = dy, db, dx, dw;
+      if (act != JLA_ACT_NONE && (need_x || need_w || need_b)) z = aligned(restored(saved[2], {rows, n}, at::kFloat, dy));
+      if (need_b || z.defined()) {
+        if (z.defined()) dz = make({rows, n}, dy.scalar_type(), dy);
         Tensor scratch;
         size_t bytes = 0;
         if (need_b) {
           bytes = abi.activation_bwd_scratch_bytes(rows, (int)n);
-          db = make({n}, at::kFloat, weight);
-          scratch = make({(int64_t)bytes}, at::kByte, weight);
+          db = make({n}, at::kFloat, dy);
+          scratch = make({(int64_t)bytes}, at::kByte, dy);
         }
-        check(abi.activation_bwd(code(weight.scalar_type()), rows, (int)n, (int)act, fptr(z), ptr(dy), z.defined() ? ptr(dz) : nullptr,
-                                 fmut(db), ptr(scratch), bytes, stream_of(weight)),
+        check(abi.activation_bwd(code(dy.scalar_type()), rows, (int)n, (int)act, fptr(z), ptr(dy), z.defined() ? ptr(dz) : nullptr,
+                                 fmut(db), ptr(scratch), bytes, stream_of(dy)),
               "jla_activation_bwd");
       }
-      if (need_x) dx = input_grad(shape, rows, dz, weight, {}, {});
-      if (need_w) weight_grads(weight, rows, x.t, x.stride, dz, dw, {}, nullptr);
+      if (need_x) dx = input_grad(shape, rows, dz, aligned(restored(saved[1], {n, depth}, dy.scalar_type(), dy)), {}, {});
+      if (need_w) weight_grads(rows_of(restored(saved[0], shape, dy.scalar_type(), dy), depth), dz, n, dw, {}, nullptr);
       out = {dx, dw, db, cfg[2] && ctx->needs_input_grad(cfg[1] ? 3 : 2) ? grads[0] : Tensor(), Tensor()};
     }
     return again ? once(out) : out;
@@ -404,7 +404,8 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     const Rows rows = rows_of(x, gate.size(1));
     Tensor g, u;
     Tensor h = gated_fwd(rows, gate, up, {}, {}, {}, act, out_shape(x, gate.size(0)), x.scalar_type(), &g, &u);
-    ctx->save_for_backward({rows.t, gate, up, g, u});
+    const bool x_too = gate.requires_grad() || up.requires_grad(), weights_too = x.requires_grad();
+    ctx->save_for_backward({x_too ? rows.t : Tensor(), weights_too ? gate : Tensor(), weights_too ? up : Tensor(), g, u});
     ctx->saved_data["act"] = act;
     ctx->saved_data["shape"] = x.sizes().vec();
     return h;
@@ -421,20 +422,23 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
       c10::cuda::OptionalCUDAGuard guard(grads[0].device());
       const Tensor dh = aligned(grads[0]);
       const int64_t depth = shape.back(), n = dh.size(-1), rows = dh.numel() / n;
-      const Rows x = rows_of(restored(saved[0], shape, dh.scalar_type(), dh), depth);
-      const Tensor gate = aligned(restored(saved[1], {n, depth}, dh.scalar_type(), dh));
-      const Tensor up = aligned(restored(saved[2], {n, depth}, dh.scalar_type(), dh));
       const Tensor g = aligned(restored(saved[3], {rows, n}, at::kFloat, dh));
       const Tensor u = aligned(restored(saved[4], {rows, n}, at::kFloat, dh));
-      const Tensor dg = make({rows, n}, gate.scalar_type(), gate), du = make({rows, n}, gate.scalar_type(), gate);
-      check(abi.gated_activation_bwd(code(gate.scalar_type()), rows, (int)n, (int)act, fptr(g), fptr(u), ptr(dh), ptr(dg), ptr(du),
-                                     stream_of(gate)),
+      const Tensor dg = make({rows, n}, dh.scalar_type(), dh), du = make({rows, n}, dh.scalar_type(), dh);
+      check(abi.gated_activation_bwd(code(dh.scalar_type()), rows, (int)n, (int)act, fptr(g), fptr(u), ptr(dh), ptr(dg), ptr(du),
+                                     stream_of(dh)),
             "jla_gated_activation_bwd");
       Tensor dx, d_gate, d_up;
       const bool need_g = ctx->needs_input_grad(1), need_u = ctx->needs_input_grad(2);
-      if (ctx->needs_input_grad(0)) dx = input_grad(shape, rows, dg, gate, du, up);
-      if (need_g) weight_grads(gate, rows, x.t, x.stride, dg, d_gate, need_u ? du : Tensor(), need_u ? &d_up : nullptr);
-      else if (need_u) weight_grads(up, rows, x.t, x.stride, du, d_up, {}, nullptr);
+      if (ctx->needs_input_grad(0)) {
+        const Tensor gate = aligned(restored(saved[1], {n, depth}, dh.scalar_type(), dh));
+        dx = input_grad(shape, rows, dg, gate, du, aligned(restored(saved[2], {n, depth}, dh.scalar_type(), dh)));
+      }
+      if (need_g || need_u) {
+        const Rows x = rows_of(restored(saved[0], shape, dh.scalar_type(), dh), depth);
+        if (need_g) weight_grads(x, dg, n, d_gate, need_u ? du : Tensor(), need_u ? &d_up : nullptr);
+        else weight_grads(x, du, n, d_up, {}, nullptr);
+      }
       out = {dx, d_gate, d_up, Tensor()};
     }
     return again ? once(out) : out;
