@@ -269,8 +269,8 @@ int jla_gated_rmsnorm_bwd(int dtype, int64_t rows, int dim, int group, const voi
  *   t = x + residual (residual may be NULL), stream_out = round(t);  y = t * rsqrt(mean(t^2) + eps) * weight
  *   out_e4m3: y is e4m3 [rows, dim] with one scale a row: scale = max |y| / 448 (1 where that is no positive normal
  *   number), y holds value / scale
- * x, residual, y, stream_out [rows, dim] dtype (any of the three); weight [dim] f32; scale [rows] f32; rstd [rows] f32 is
- * written for the backward call, or NULL. 1 <= dim <= 16384.
+ * x, residual, y, stream_out [rows, dim] dtype (any of the three); stream_out may be NULL where residual is; weight [dim]
+ * f32; scale [rows] f32; rstd [rows] f32 is written for the backward call, or NULL. 1 <= dim <= 16384.
  * Backward: x, residual, weight as forward; dy, dstream (NULL = zero) and dx [rows, dim] dtype; dx is the gradient of x and
  * of the residual alike; dweight [dim] f32 or NULL; scratch of jla_rms_norm_bwd_scratch_bytes() where
  * dweight is wanted. Sums are taken in the same order every time. */

@@ -228,6 +228,8 @@ __global__ void __launch_bounds__(1024) rms_norm_fwd_kernel(RmsParams p) {
       float r[VEC];
       rr[j].get(r);
       add_to<VEC>(f[j], r);
+    }
+    if (p.stream) {
       const int c = (j * tpr + threadIdx.x) * VEC;
       if (live && c < p.dim) R::store(static_cast<T*>(p.stream) + base + c, f[j]);
     }
