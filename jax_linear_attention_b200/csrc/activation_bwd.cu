@@ -5,7 +5,9 @@
 //
 // Bound by HBM: z (or g and u) is read in float32, dy and the results are 16-bit. The forward pass keeps z in float32, not
 // in 16 bits, because its rounding would come on top of the one of dz, which the tensor cores cannot do without; a 16-bit
-// z makes dx half as far again from the exact gradient for 2 bytes an element fewer.
+// z makes dx half as far again from the exact gradient for 2 bytes an element fewer. What the rounding of dz, dg and du costs: dx and
+// dW are 2.9e-4 instead of 2.1e-4 off in f16 (4096 x 2048 x 2048 with sigmoid), 2.3e-3 instead of 1.7e-3 in bf16 (gated 16384 x
+// 2048 x 5632), as torch's own gradients of these types are; two 16-bit halves of each would keep it at twice the products.
 //
 // Measured on a B200: gated 16384 x 5632 bf16 188 us (6.7 TB/s); 4096 x 2048 f16 with dbias 12 + 3 us.
 //

@@ -25,9 +25,9 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
-// One-instruction approximations for the element-wise kernels (relative error about 2^-22: far below the rounding of
-// 16-bit outputs and inside the 1e-5 their float32 paths are held to); the IEEE-rounded reciprocal, the division and
-// the library exp / log cost ten to thirty instructions each.
+// One-instruction approximations for the element-wise kernels (relative error about 2^-22, of fast_exp(x) about |x| 2^-23 more,
+// since x log2 e is rounded first: far below the rounding of 16-bit outputs, and inside the 1e-5 that their float32 paths are held
+// to); the IEEE-rounded reciprocal, the division and the library exp / log cost ten to thirty instructions each.
 __device__ __forceinline__ float fast_rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -8,9 +8,10 @@
 // shared memory, and add the parts up in the order of the parts, every time the same. A CTA with more than kPartSteps steps of
 // its own sums those in runs of as many, one after the other in the same accumulator, and joins them in a second one.
 //
-// Measured on a B200, weights from HBM: one token, 2048 -> 8512 bf16 8.2 us (35 MB; 5.3 at HBM's rate); 33 tokens, 4096 -> 2048 e4m3
-// 6.5 us; gated, four tokens, 2048 -> 5632 bf16 8.8 us warm, 13 us from HBM (46 MB). Of that about 0.8 us are set-up, 1.5 to 2.5 us
-// the way of the first bytes, 1.5 to 2 us the sums and results.
+// Measured on a B200, weights from HBM, one pass among others (a kernel starts under the end of the one before; by itself it takes
+// about 4 us more): one token, 2048 -> 8512 bf16 9.3 us (35 MB; 5.3 at HBM's rate); 33 tokens, 4096 -> 2048 e4m3 6.6 us; gated, four
+// tokens, 2048 -> 5632 bf16 10.9 us (46 MB; 7.1). Of that about 0.8 us are set-up, 1.5 to 2.5 us the way of the first bytes, 1.5 to
+// 2 us the sums and results.
 //
 // Every wait is bounded, as in product_tc.cu (kStatusFewTokens).
 #include "overlap.cuh"
@@ -49,8 +50,10 @@ template <int BN, bool GATED> struct Shape {
   // Partial sums that arrive: whole rounds of up to eight parts, [weight][part][token][128 features].
   static constexpr int kPartRows = BN + kMaxSplit, kPartBytes = kWeights * kPartRows * 512;
   // The ring of operand tiles; afterwards this CTA's own partial sums, [weight][token][128 features]. Half an SM's memory where
-  // one weight's sums leave enough of it for the ring: the next kernel's CTAs are set up beside this one's, and a CTA alone
-  // needs no deeper ring (one token, 2048 -> 8512: 12.6 us, with all of the memory 13.2).
+  // one weight's sums leave enough of it for the ring: the next kernel's CTAs are set up beside this one's, and two CTAs of a wide
+  // product have room. (A pass among others, with all of the memory in brackets: one token, 2048 -> 32768 22.5 us (26.7),
+  // 4096 -> 2048 6.6 (6.9), 2048 -> 8512 9.2 (9.3; 9.1 where torch allocates between the passes); but 32 tokens, 2048 -> 8512 10.6 (10.0),
+  // and 20 tokens, 8192 -> 8192 27.3 (24.9).)
   static constexpr int kCtas = !GATED && BN <= 32 ? 2 : 1;
   static constexpr int kRoom = (kCtas == 2 ? 110 : 224) * 1024 - 1024 - kPartBytes;
   static constexpr int kFit = kRoom / kStageBytes;
@@ -421,12 +424,15 @@ int pick(const Product& p, int dev, cudaStream_t s) {
 }  // namespace
 
 // Up to 64 tokens always; up to 8192 where this kernel is expected to be the faster one. Fitted, in hundredths of a us with
-// inputs from HBM, to times of both from 33 to 1500 tokens, depths of 64 to 4096 and widths of 256 to 6144:
+// inputs from HBM, to times of both in bf16 and f16 from 33 to 1500 tokens, depths of 64 to 4096 and widths of 256 to 6144:
 //   this kernel: 200 + waves (390 + 36 a step of the longest CTA), 110 more where the contraction is split (gated 360, 48, 160)
 //   pairs: 720 + 20 a step of the busiest pair; an activation or bias shows with 290 (here 30), a residual with 200 (here 100)
 // Some of the times, in us, this kernel against pairs of CTAs: 4096 -> 256, 512 tokens: 10.7, 18.7; 4096 -> 2048, 256: 14.5,
 // 20.2; 512 -> 512, 256: 7.9, 9.6, with silu and a residual 8.4, 15.2; 2048 -> 6144, 256: 18.6, 14.8; gated 2048 -> 6144, 256:
 // 40.9, 21.3; gated 64 -> 256, 1500: 5.5, 7.6.
+// Beyond what it was fitted to (546 calls of 65 to 8192 tokens, depths of 64 to 16384, widths of 64 to 8192, e4m3, dx and gated
+// among them) it takes the kernel that is slower by more than 15 % in 18 cases: e4m3 with 64 features (13 us, 10 with pairs),
+// and sums over 8192 and more at 4000 tokens and 256 features (74 us with pairs, 64 here).
 bool few_tokens_applies(const Product& p, int sms) {
   if (p.x_mn || p.group || p.rows > 8192) return false;
   if (p.rows <= 64) return true;

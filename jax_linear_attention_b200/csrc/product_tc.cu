@@ -14,9 +14,9 @@
 // Tiles of a last round that would leave more than half of the pairs idle are taken in halves (1003 x 2048 x 6144 f16, 96
 // tiles on 74 pairs: 31 -> 27 us with silu; 700 x 2048 x 2048, 24 tiles: 19.5 -> 15.7 us).
 //
-// Measured on a B200, inputs from HBM: 16384 x 4096 x 2048 bf16 163 us forward, 165 us dx, 177 us dW (128 tiles on 74 pairs; cuBLAS
-// 178, 169, 168); gated 16384 x 2048 x 5632 bf16 460 us, 532 us with g and u kept; gated 5003 x 2048 x 5632 e4m3 81 us. The tensor
-// pipe is active 79 to 95 % of the time. A step of the contraction takes 512 cycles of the tensor core and as much of what an SM
+// Measured on a B200, inputs from HBM, each launch by itself: 16384 x 4096 x 2048 bf16 163 us forward, 165 us dx, 177 us dW (128 tiles on 74 pairs; cuBLAS
+// 178, 169, 168); gated 16384 x 2048 x 5632 bf16 460 us, 532 us with g and u kept; gated 5003 x 2048 x 5632 e4m3 81 us. In a row of
+// steps the power limit adds up to a third. The tensor pipe is active 73 to 95 % of the time. A step of the contraction takes 512 cycles of the tensor core and as much of what an SM
 // can read from L2 (64 bytes a cycle), so that neither waits for the other by much.
 //
 // Where the operands end inside a tile TMA reads zeros and its stores leave out what lies beyond. No load is multicast.
@@ -274,8 +274,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       if (lane == 0) umma::arrive_cluster(umma::map_rank(smem_addr(acc_empty + a), 0));
     };
     // A long contraction: its parts come one after the other in the first accumulator, their sum is kept in the second, each
-    // column by the warp that needs it in the end. (The products stand still while a part is taken over, which does not show: dW of 65536 x 2048 x 2048 345 us
-    // with and without.)
+    // column by the warp that needs it in the end. (The products stand still while a part is taken over, which does not show: dW
+    // of 65536 x 2048 x 2048 345 us with and without.)
     int joined = 0;
     auto join = [&](int cols, uint32_t sum) {
       for (int k0 = 0; k0 < p.kt; k0 += p.part, ++joined) {

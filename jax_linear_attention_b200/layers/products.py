@@ -14,7 +14,9 @@ that the gradient of a weight sums over.
 
 Forward is one launch, of a kernel for many tokens or of one for few (``csrc/product_tc.cu``, ``csrc/few_tokens.cu``).
 Backward, ``dx`` and ``dW`` are one launch each (both halves of a gated block together), after one for the activation's
-gradient and the bias's where there are any. Before an activation the product is kept in float32 for the backward pass.
+gradient and the bias's where there are any. Before an activation the product is kept in float32 for the backward pass; the
+activation's gradient is rounded to the operands' type before the products (half a step more in ``dx`` and ``dW``). Only what the
+wanted gradients read is kept.
 A backward pass is captured into a graph like any other work, but not while an eager autograd graph of its leaves is alive on the
 default stream, nor where a part of its graph was made there (a weight that was transposed before the capture): that raises.
 """
