@@ -80,7 +80,8 @@ def _build_torch_ops(force: bool, verbose: bool) -> None:
     import torch
 
     cmd = _torch_ops_command()
-    made_by, note = dict(torch=torch.__version__, python=sys.version, command=cmd), os.path.join(OBJ, "_torch_ops.json")
+    command = [part.replace(HERE, "") for part in cmd]  # (the tree may be moved with what was built in it)
+    made_by, note = dict(torch=torch.__version__, python=sys.version, command=command), os.path.join(OBJ, "_torch_ops.json")
     try:
         with open(note) as f:
             same = json.load(f) == made_by
