@@ -101,6 +101,8 @@ def rms_norm(x, weight, *, residual=None, eps: float = 1e-6, out_dtype=None):
     if not isinstance(weight, torch.Tensor) or weight.shape != x.shape[-1:] or weight.device != x.device or not weight.is_floating_point():
         raise ValueError(f"weight must be a floating [{x.shape[-1]}] on {x.device}; got "
                          f"{weight if not isinstance(weight, torch.Tensor) else (weight.dtype, tuple(weight.shape), weight.device)}")
+    if residual is not None and not isinstance(residual, torch.Tensor):
+        raise ValueError(f"residual must be a tensor or None; got {type(residual).__name__}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError(f"residual must be {x.dtype} {tuple(x.shape)} on {x.device}; got {residual.dtype} "
                          f"{tuple(residual.shape)} on {residual.device}")

@@ -38,6 +38,12 @@ def _code(name: str, activation, allowed) -> int:
     return _ACTIVATIONS[activation]
 
 
+def _no_tensor(name: str, **operands):
+    for label, t in operands.items():
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name}: {label} must be a tensor or None; got {type(t).__name__}")
+
+
 def _refuse(name: str, x, weights, scales, x_scale, out_dtype):
     """Says what keeps ``csrc/torch_ops.cpp`` from taking these operands; returns the output's dtype where nothing does."""
     for label, t in (("x", x), *((f"weight {i}", w) for i, w in enumerate(weights))):
@@ -86,6 +92,7 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
     y = (_lib._torch_ops or _lib.torch_ops()).linear(x, weight, bias, act, residual, x_scale, weight_scale, out_dtype)
     if y is not None:
         return y
+    _no_tensor("linear", bias=bias, residual=residual, x_scale=x_scale, weight_scale=weight_scale)
     dtype = _refuse("linear", x, (weight,), (weight_scale,), x_scale, out_dtype)
     shape = (*x.shape[:-1], weight.shape[0])
     if bias is not None and (bias.shape != weight.shape[:1] or bias.device != x.device or not bias.is_floating_point()):
@@ -107,5 +114,6 @@ def gated_linear(x, w_gate, w_up, *, activation: str = "silu", x_scale=None, gat
     h = (_lib._torch_ops or _lib.torch_ops()).gated_linear(x, w_gate, w_up, act, x_scale, gate_scale, up_scale, out_dtype)
     if h is not None:
         return h
+    _no_tensor("gated_linear", x_scale=x_scale, gate_scale=gate_scale, up_scale=up_scale)
     _refuse("gated_linear", x, (w_gate, w_up), (gate_scale, up_scale), x_scale, out_dtype)
     raise ValueError("gated_linear: e4m3 operands have no gradient: call it under torch.no_grad()")

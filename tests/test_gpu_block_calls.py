@@ -119,3 +119,18 @@ def test_compiled_around():
     y = compiled(x)
     got = torch.autograd.grad(y, [x, *block.parameters()], dy)
     assert bool((y == want).all()) and all(bool((a == b).all()) for a, b in zip(got, grads))
+
+
+def test_operands_that_are_no_tensors():
+    x, w, n = _normal(8, 64), _normal(72, 64), torch.ones(64, device="cuda")
+    q, s, qs = x.to(torch.float8_e4m3fn), torch.ones(8, device="cuda"), torch.ones(72, device="cuda")
+    qw = w.to(torch.float8_e4m3fn)
+    for call, text in ((lambda: layers.linear(x, w, 0.5), "bias"), (lambda: layers.linear(x, w, residual=[1.0]), "residual"),
+                       (lambda: layers.linear(q, qw, x_scale=1.0, weight_scale=qs), "x_scale"),
+                       (lambda: layers.linear(q, qw, x_scale=s, weight_scale=1.0), "weight_scale"),
+                       (lambda: layers.gated_linear(q, qw, qw, x_scale=s, gate_scale=qs, up_scale=2), "up_scale"),
+                       (lambda: layers.rms_norm(x, n, residual=0), "residual"), (lambda: layers.rms_norm(x, 1.0), "weight"),
+                       (lambda: layers.linear(x, None), "weight 0"), (lambda: layers.gated_linear(x, w, None), "weight 1"),
+                       (lambda: layers.linear(x, w, out_dtype="bf16"), "out_dtype")):
+        with pytest.raises(ValueError, match=text):
+            call()
